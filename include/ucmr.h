@@ -55,6 +55,11 @@ extern "C" {
 #define UCMR_DEV_WAIT_TIMEOUT 2 /* a bounded wait inside a kernel gave up                        */
 #define UCMR_DEV_BAD_SLOT 4     /* reserved                                                      */
 
+/* Element types of the operators that take more than one (rotary positions, cache append, attention). */
+#define UCMR_BF16 0
+#define UCMR_FP16 1
+#define UCMR_E4M3 2 /* 8-bit codes: sign, 4 exponent bits, 3 mantissa bits, no infinities, largest 448 */
+
 #define UCMR_REDUCE_MIN 0 /* block score = min over tokens (reference behaviour)                 */
 #define UCMR_REDUCE_SUM 1 /* block score = sum over tokens (mean * BS * G)                       */
 /* May be OR-ed into reduce_mode: the caller guarantees that seq_lens and block_table are NOT written by any
@@ -405,6 +410,78 @@ size_t ucmr_softmax_topk_workspace_bytes(int X, int Hq, int n_blocks, int M);
 int ucmr_softmax_topk(const void* repr, int n_blocks, int M, int Hkv, int D, const void* q, int X, int Hq, int k,
                       float* out_block_scores, float* out_scores, int32_t* out_ids, void* workspace,
                       size_t workspace_bytes, void* stream);
+
+/* ---------------------------------------------------------------------------------------------
+ *  Filling the paged KV cache and attending over it (no counterpart in the reference, which leaves both to its
+ *  engine): rotary positions, the append of a step's keys and values, attention over the blocks of a table -
+ *  for example the out_physical / out_new_seq_lens of ucmr_hamming_topk.
+ *
+ *  ucmr_rotary: x, out bf16 or fp16 [T, H, D] (strides in elements, unit inner stride; out may be x itself, any other
+ *     overlap is not allowed).  On the first rotary_dim elements of a head, pair i - elements (i, i + rotary_dim/2), or
+ *     (2i, 2i+1) when interleaved - becomes
+ *         mscale * (a cos - b sin, b cos + a sin) of the angle positions[t] * inv_freq[i],
+ *     with the angle negated when transpose != 0 (the transposed map: the gradient, and for mscale = 1 the inverse);
+ *     the other elements are copied.  positions int32 or int64 [T], any value; inv_freq float64 [rotary_dim/2] (device,
+ *     radians per position; scalings for long contexts go in here and in mscale).  Angles are reduced exactly (64-bit
+ *     fractions of a turn): the error of an angle is at most |positions * inv_freq| * 2^-53 + 2^-23.
+ *     float32 arithmetic, one rounding.
+ * ------------------------------------------------------------------------------------------ */
+int ucmr_rotary(const void* x, void* out, int64_t T, int H, int D, int64_t x_stride_t, int64_t x_stride_h,
+                int64_t out_stride_t, int64_t out_stride_h, int dtype, const void* positions, int pos_is_int64,
+                const double* inv_freq, int rotary_dim, int interleaved, float mscale, int transpose, void* stream);
+
+/*  ucmr_kv_append: token t's key and value rows k[t], v[t] (bf16 or fp16 [T, Hkv, D], strides in elements) go to slot
+ *     slot_mapping[t] (= block*BS + row; int32 or int64) of k_cache / v_cache [NB, BS, Hkv, D] (strides in elements).
+ *     Slots < 0 or >= NB*BS are skipped; of two tokens with the same slot the later one is stored.  With inv_freq the
+ *     keys are rotated first (as ucmr_rotary, transpose = 0; positions [T]).
+ *     cache_dtype = dtype: the rows themselves (k_scale = v_scale = NULL).
+ *     cache_dtype = UCMR_E4M3: codes, value = code * scale[block, head], float32 scales [NB, Hkv] (>= 0).  The scale is the
+ *       smallest power of two >= 2^-126 with 448 * scale >= the largest finite magnitude of the block and head, 0 if all
+ *       are 0.  A call that writes row 0 of a block starts the block anew: rows that it does not write keep their codes
+ *       and lose their value.  Otherwise the scale becomes the larger of the stored one and the one that the new rows
+ *       need; if it grows, the codes of the other rows are re-rounded to it.  Values that are not finite are stored as
+ *       NaN and have no say in the scale.
+ *     q (may be NULL): the step's queries [T, Hq, D], rotated into q_out (may be q).  k_out (may be NULL, not k): the rotated
+ *     keys of all T tokens in 16 bits [T, Hkv, D], for example for ucmr_hash_encode_decode_step.  Both need inv_freq.
+ *     D a multiple of 16 up to 512, BS up to 1024, rotary_dim a multiple of 16; k, v and the caches 16-byte aligned with
+ *     strides of whole 16-byte vectors.
+ * ------------------------------------------------------------------------------------------ */
+int ucmr_kv_append(const void* k, int64_t k_stride_t, int64_t k_stride_h, const void* v, int64_t v_stride_t,
+                   int64_t v_stride_h, int64_t T, int Hkv, int D, int dtype, const void* slot_mapping, int slot_is_int64,
+                   void* k_cache, int64_t kc_stride_block, int64_t kc_stride_t, int64_t kc_stride_h, void* v_cache,
+                   int64_t vc_stride_block, int64_t vc_stride_t, int64_t vc_stride_h, int64_t NB, int BS, int cache_dtype,
+                   float* k_scale, float* v_scale, const void* positions, int pos_is_int64, const double* inv_freq,
+                   int rotary_dim, int interleaved, float mscale, const void* q, int Hq, int64_t q_stride_t,
+                   int64_t q_stride_h, void* q_out, int64_t qo_stride_t, int64_t qo_stride_h, void* k_out,
+                   int64_t ko_stride_t, int64_t ko_stride_h, void* stream);
+
+/*  ucmr_paged_attention: out[t, head] = sum_p softmax_p(scale * <q[t, head], k[p]>) v[p] over the tokens p of the request
+ *     that token t belongs to.  q, out bf16 or fp16 [T, Hq, D]; caches and scales as above (cache_dtype = dtype or
+ *     UCMR_E4M3); head h uses kv head h / (Hq / Hkv).  Token p of request b lies in row p % BS of block
+ *     block_table[b * bt_stride_b + kv_head * bt_stride_h + p / BS] (bt_stride_h = 0: one list for all kv heads; Hkv lists
+ *     as a per-head retrieval returns them); its length is seq_lens[b], cut to max_blocks*BS.
+ *     Request b has the query tokens [query_start[b], query_start[b+1]) of q (int32 [B+1], ascending), or token b when
+ *     query_start is NULL (then T = B).  They are its last tokens: with causal != 0, query i of n sees the first
+ *     seq_lens[b] - n + 1 + i tokens, without it all.  A row that sees nothing becomes 0 with log-sum-exp -inf; rows of q
+ *     and out outside every request are neither read nor written.  max_query_len >= the largest n picks the kernel.
+ *     lse (may be NULL): float32 [T, Hq], natural logarithm of the sum of exp(scale * score): partial results over
+ *     disjoint blocks (a sequence-sharded cache) are merged with it.
+ *     Tokens of blocks outside [0, NB) are left out and flagged (UCMR_DEV_BAD_BLOCK_ID) in the workspace's status word.
+ *     Values in masked places (behind a length, above the diagonal) never reach a result, NaN included.
+ *     D is 64 or 128.  q, out, caches: 16-byte aligned, strides of whole 16-byte vectors.
+ *     workspace: ucmr_paged_attention_workspace_bytes(D) bytes, cleared once with ucmr_paged_attention_workspace_init (or
+ *     zero-filled); calls that may overlap on the GPU need different workspaces.  Results do not depend on timing.
+ * ------------------------------------------------------------------------------------------ */
+size_t ucmr_paged_attention_workspace_bytes(int head_dim);
+int ucmr_paged_attention_workspace_init(void* workspace, size_t bytes, void* stream);
+int ucmr_paged_attention(const void* q, int64_t T, int Hq, int D, int64_t q_stride_t, int64_t q_stride_h, int dtype,
+                         const void* k_cache, int64_t kc_stride_block, int64_t kc_stride_t, int64_t kc_stride_h,
+                         const void* v_cache, int64_t vc_stride_block, int64_t vc_stride_t, int64_t vc_stride_h, int64_t NB,
+                         int BS, int Hkv, int cache_dtype, const float* k_scale, const float* v_scale,
+                         const int32_t* block_table, int max_blocks, int64_t bt_stride_b, int64_t bt_stride_h,
+                         const int32_t* seq_lens, const int32_t* query_start, int max_query_len, int B, float scale,
+                         int causal, void* out, int64_t o_stride_t, int64_t o_stride_h, float* lse, void* workspace,
+                         size_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }

@@ -12,7 +12,9 @@ PKG_DIR = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(PKG_DIR, "csrc")
 INCLUDE = os.path.join(os.path.dirname(PKG_DIR), "include")
 LIB_PATH = os.path.join(PKG_DIR, "libucmr_b200.so")
-SOURCES = ["api.cu", "scan.cu", "scan_ring.cu", "scan_rows.cu", "topk.cu", "gather.cu", "encode.cu", "noalloc.cu", "float_retrieval.cu"]
+SOURCES = ["api.cu", "scan.cu", "scan_ring.cu", "scan_rows.cu", "topk.cu", "gather.cu", "encode.cu", "noalloc.cu", "float_retrieval.cu",
+           "rotary.cu", "kv_append.cu", "paged_attention.cu"]
+HEADERS = ["common.cuh", "rotary.cuh", "paged_attention.cuh"]
 
 
 def _sources():
@@ -20,7 +22,7 @@ def _sources():
 
 
 def _deps():
-    deps = _sources() + [os.path.join(CSRC, "common.cuh"), os.path.join(INCLUDE, "ucmr.h")]
+    deps = _sources() + [os.path.join(CSRC, h) for h in HEADERS] + [os.path.join(INCLUDE, "ucmr.h")]
     return [d for d in deps if os.path.exists(d)]
 
 

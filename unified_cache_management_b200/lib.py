@@ -17,6 +17,8 @@ UCMR_ERR_WORKSPACE = -5
 UCMR_DEV_BAD_BLOCK_ID = 1
 UCMR_DEV_WAIT_TIMEOUT = 2
 
+BF16, FP16, E4M3 = 0, 1, 2
+
 REDUCE_MIN = 0
 REDUCE_SUM = 1
 
@@ -81,6 +83,15 @@ SIGNATURES = {
                                            C.POINTER(C.c_void_p), C.POINTER(C.c_void_p), _i, _vp, _vp, _sz, _vp]),
     "ucmr_merge_topk_wait_step": (_i, [_vp, _vp, _i64, _i64, _i, _i, _i, _i, _i, _vp, _vp, _vp, _i64, _vp, _vp, _vp, _vp]),
     "ucmr_copy_blocks": (_i, [_vp, _vp, _vp, _vp, _i64, _i64, _vp, _vp]),
+    "ucmr_rotary": (_i, [_vp, _vp, _i64, _i, _i, _i64, _i64, _i64, _i64, _i, _vp, _i, _vp, _i, _i, _f, _i, _vp]),
+    "ucmr_kv_append": (_i, [_vp, _i64, _i64, _vp, _i64, _i64, _i64, _i, _i, _i, _vp, _i, _vp, _i64, _i64, _i64, _vp, _i64, _i64,
+                            _i64, _i64, _i, _i, _vp, _vp, _vp, _i, _vp, _i, _i, _f, _vp, _i, _i64, _i64, _vp, _i64, _i64, _vp,
+                            _i64, _i64, _vp]),
+    "ucmr_paged_attention_workspace_bytes": (_sz, [_i]),
+    "ucmr_paged_attention_workspace_init": (_i, [_vp, _sz, _vp]),
+    "ucmr_paged_attention": (_i, [_vp, _i64, _i, _i, _i64, _i64, _i, _vp, _i64, _i64, _i64, _vp, _i64, _i64, _i64, _i64, _i, _i,
+                                  _i, _vp, _vp, _vp, _i, _i64, _i64, _vp, _vp, _i, _i, _f, _i, _vp, _i64, _i64, _vp, _vp, _sz,
+                                  _vp]),
     "ucmr_gather_kv": (_i, [_vp, _vp, _i64, _i64, _vp, _i, _i, _i, _i, _i, _i64, _vp, _vp, _vp, _vp]),
 }
 

@@ -6,7 +6,9 @@ is no PyTorch or CPU implementation behind these functions.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes as C
+import math
 from dataclasses import dataclass
 from typing import Optional, Sequence
 
@@ -773,3 +775,293 @@ def softmax_topk(repr_blocks: torch.Tensor, q: torch.Tensor, k: int, workspace: 
                                    _ptr(scores), _ptr(ids), _ptr(workspace), workspace.numel(), _stream(q)),
              "ucmr_softmax_topk")
     return block_scores, scores, ids
+
+
+# ----------------------------------------------------------------------------------------------
+# the paged KV cache itself: rotary positions, append, attention
+# ----------------------------------------------------------------------------------------------
+_TYPES = {torch.bfloat16: _l.BF16, torch.float16: _l.FP16, torch.float8_e4m3fn: _l.E4M3}
+_ROPE_TYPES = ("default", "linear", "dynamic", "llama3", "yarn")
+
+
+def rotary_frequencies(rotary_dim: int, base: float = 10000.0, scaling: Optional[dict] = None, device=None):
+    """(inv_freq float64 [rotary_dim/2], mscale) of a model's ``rope_theta`` and ``rope_scaling`` entry: ``rope_type``
+    (or ``type``) 'default', 'linear' (factor), 'dynamic' (factor, original_max_position_embeddings, seq_len: the base
+    grows with a length beyond the original one), 'llama3' (factor, low_freq_factor, high_freq_factor,
+    original_max_position_embeddings) or 'yarn' (factor, original_max_position_embeddings, beta_fast, beta_slow,
+    attention_factor)."""
+    if rotary_dim <= 0 or rotary_dim % 2:
+        raise ValueError("rotary_dim must be even and positive")
+    cfg = dict(scaling or {})
+    kind = cfg.get("rope_type", cfg.get("type", "default"))
+    if kind not in _ROPE_TYPES:
+        raise ValueError(f"rope type should be one of {_ROPE_TYPES}, got {kind!r}")
+    i = torch.arange(rotary_dim // 2, dtype=torch.float64)
+    if kind == "default":
+        return (base ** (-2.0 * i / rotary_dim)).to(device), 1.0
+    factor = float(cfg["factor"])
+    if factor <= 0:
+        raise ValueError("the rope scaling factor must be positive")
+    mscale = 1.0
+    if kind == "dynamic":
+        original = float(cfg["original_max_position_embeddings"])
+        ratio = max(float(cfg.get("seq_len", original)), original) / original
+        base = base * (factor * ratio - (factor - 1.0)) ** (rotary_dim / (rotary_dim - 2.0)) if rotary_dim > 2 else base
+        return (base ** (-2.0 * i / rotary_dim)).to(device), mscale
+    f = base ** (-2.0 * i / rotary_dim)
+    if kind == "linear":
+        f = f / factor
+    elif kind == "llama3":
+        # pairs that turn more than high_freq_factor times over the original context keep their frequency, those that
+        # turn less than low_freq_factor times are slowed by the factor, the ones between are blended
+        lo, hi = float(cfg.get("low_freq_factor", 1.0)), float(cfg.get("high_freq_factor", 4.0))
+        turns = float(cfg["original_max_position_embeddings"]) * f / (2.0 * math.pi)
+        keep = ((turns - lo) / (hi - lo)).clamp(0.0, 1.0)
+        f = f * (keep + (1.0 - keep) / factor)
+    else:
+        original = float(cfg["original_max_position_embeddings"])
+
+        def pair_with(turns):  # (fractional) pair that turns this often over the original context
+            return rotary_dim * math.log(original / (2.0 * math.pi * turns)) / (2.0 * math.log(base))
+        first = max(math.floor(pair_with(float(cfg.get("beta_fast", 32.0)))), 0)
+        last = min(math.ceil(pair_with(float(cfg.get("beta_slow", 1.0)))), rotary_dim - 1)
+        slow = ((i - first) / max(last - first, 0.001)).clamp(0.0, 1.0)
+        f = f * (1.0 - slow) + f / factor * slow
+        mscale = cfg.get("attention_factor")
+        mscale = float(mscale) if mscale is not None else (0.1 * math.log(factor) + 1.0 if factor > 1 else 1.0)
+    return f.to(device), mscale
+
+
+def _type_of(name: str, t: torch.Tensor, allowed) -> int:
+    if not isinstance(t, torch.Tensor) or not t.is_cuda:
+        raise ValueError(f"{name} must be a CUDA tensor")
+    if t.dtype not in allowed:
+        raise ValueError(f"{name} must have dtype {' or '.join(str(a) for a in allowed)}, got {t.dtype}")
+    return _TYPES[t.dtype]
+
+
+_ACTIVATIONS = (torch.bfloat16, torch.float16)
+_INDEXES = (torch.int64, torch.int32)
+
+
+def _heads(name: str, t: torch.Tensor, dims: int = 3) -> None:
+    if t.dim() != dims or (t.stride(-1) != 1 and t.shape[-1] != 1):
+        raise ValueError(f"{name} must have {dims} dimensions with a unit inner stride, got {tuple(t.shape)}, strides {t.stride()}")
+
+
+def _same_device(device, **tensors) -> None:
+    for name, t in tensors.items():
+        if t is not None and t.device != device:
+            raise ValueError(f"{name} is on {t.device}, the others are on {device}")
+
+
+def _raw_stream(device) -> int:
+    return torch._C._cuda_getCurrentRawStream(device.index)
+
+
+def _on(device):
+    """Makes the tensors' device the current one for the launch."""
+    return torch.cuda.device(device) if torch.cuda.current_device() != device.index else contextlib.nullcontext()
+
+
+def _angles(positions, inv_freq, tokens: int, dim: int):
+    if inv_freq is None or positions is None:
+        raise ValueError("positions and inv_freq are given together")
+    _need_cuda("inv_freq", inv_freq, torch.float64)
+    _need_cuda("positions", positions, _INDEXES)
+    if inv_freq.dim() != 1 or inv_freq.numel() == 0 or 2 * inv_freq.numel() > dim:
+        raise ValueError(f"inv_freq must have between 1 and {dim // 2} entries, got {tuple(inv_freq.shape)}")
+    if positions.shape != (tokens,):
+        raise ValueError(f"positions must be [{tokens}], got {tuple(positions.shape)}")
+    return 2 * inv_freq.numel()
+
+
+def rotary(x: torch.Tensor, positions: torch.Tensor, inv_freq: torch.Tensor, *, interleaved: bool = False,
+           mscale: float = 1.0, transpose: bool = False, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Rotates the first 2 * len(inv_freq) elements of every head of x [T, H, D] (bf16 / fp16) by positions[t] *
+    inv_freq; see ``ucmr_rotary``.  ``out`` may be x itself.  ``transpose`` applies the transposed map, which takes the
+    gradient of the output to the gradient of x."""
+    dt = _type_of("x", x, _ACTIVATIONS)
+    _heads("x", x)
+    t, h, d = x.shape
+    rot = _angles(positions, inv_freq, t, d)
+    if out is None:
+        out = torch.empty((t, h, d), dtype=x.dtype, device=x.device)
+    elif out is not x:
+        if _type_of("out", out, (x.dtype,)) != dt or out.shape != x.shape:
+            raise ValueError(f"out must be like x: {tuple(x.shape)}, got {tuple(out.shape)}")
+        _heads("out", out)
+    _same_device(x.device, out=out, positions=positions, inv_freq=inv_freq)
+    with _on(x.device):
+        _l.check(_l.load_library().ucmr_rotary(
+            x.data_ptr(), out.data_ptr(), t, h, d, x.stride(0), x.stride(1), out.stride(0), out.stride(1), dt,
+            positions.data_ptr(), positions.dtype == torch.int64, inv_freq.data_ptr(), rot, bool(interleaved),
+            float(mscale), bool(transpose), _raw_stream(x.device)), "ucmr_rotary")
+    return out
+
+
+def _check_cache(k_cache, v_cache, k_scale, v_scale, dtype, hkv: int, d: int) -> int:
+    """Element type of the two caches [NB, BS, Hkv, D]; scales [NB, Hkv] with e4m3 codes and only then."""
+    kind = _type_of("k_cache", k_cache, (dtype, torch.float8_e4m3fn))
+    if _type_of("v_cache", v_cache, (k_cache.dtype,)) != kind or v_cache.shape != k_cache.shape:
+        raise ValueError("k_cache and v_cache must agree in shape and dtype")
+    for name, c in (("k_cache", k_cache), ("v_cache", v_cache)):
+        _heads(name, c, 4)
+        if c.shape[2] != hkv or c.shape[3] != d:
+            raise ValueError(f"{name} must be [NB, BS, {hkv}, {d}], got {tuple(c.shape)}")
+    for name, s in (("k_scale", k_scale), ("v_scale", v_scale)):
+        if (s is None) == (kind == _l.E4M3):
+            raise ValueError(f"{name} belongs to a cache of e4m3 codes, and such a cache needs it")
+        if s is not None:
+            _need_cuda(name, s, torch.float32)
+            if s.shape != (k_cache.shape[0], hkv):
+                raise ValueError(f"{name} must be [{k_cache.shape[0]}, {hkv}], got {tuple(s.shape)}")
+    return kind
+
+
+def kv_append(k: torch.Tensor, v: torch.Tensor, slot_mapping: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
+              *, k_scale: Optional[torch.Tensor] = None, v_scale: Optional[torch.Tensor] = None,
+              positions: Optional[torch.Tensor] = None, inv_freq: Optional[torch.Tensor] = None,
+              interleaved: bool = False, mscale: float = 1.0, q: Optional[torch.Tensor] = None,
+              q_out: Optional[torch.Tensor] = None, k_out: Optional[torch.Tensor] = None) -> Optional[torch.Tensor]:
+    """Stores a step's keys and values [T, Hkv, D] in their slots of the paged caches [NB, BS, Hkv, D], in one launch.
+
+    With ``inv_freq`` (and ``positions``) the keys are rotated on the way, the queries ``q`` [T, Hq, D] into ``q_out`` (which
+    is returned; made if None), and the rotated keys also go to ``k_out`` in 16 bits (for the hash encode).  Caches of
+    k's dtype hold the rows; caches of float8_e4m3fn hold codes, with ``k_scale`` / ``v_scale`` float32 [NB, Hkv].  See
+    ``ucmr_kv_append`` for how a block's scale starts and grows."""
+    dt = _type_of("k", k, _ACTIVATIONS)
+    if _type_of("v", v, (k.dtype,)) != dt or v.shape != k.shape:
+        raise ValueError("k and v must agree in shape and dtype")
+    _heads("k", k)
+    _heads("v", v)
+    t, hkv, d = k.shape
+    kind = _check_cache(k_cache, v_cache, k_scale, v_scale, k.dtype, hkv, d)
+    _need_cuda("slot_mapping", slot_mapping, _INDEXES)
+    if slot_mapping.shape != (t,):
+        raise ValueError(f"slot_mapping must be [{t}], got {tuple(slot_mapping.shape)}")
+    rot = 0
+    if inv_freq is not None or positions is not None:
+        rot = _angles(positions, inv_freq, t, d)
+    elif q is not None or k_out is not None:
+        raise ValueError("q and k_out need positions and inv_freq")
+    hq = 0
+    if q is not None:
+        _type_of("q", q, (k.dtype,))
+        _heads("q", q)
+        if q.shape[0] != t or q.shape[2] != d:
+            raise ValueError(f"q must be [{t}, Hq, {d}], got {tuple(q.shape)}")
+        hq = q.shape[1]
+        if q_out is None:
+            q_out = torch.empty((t, hq, d), dtype=q.dtype, device=q.device)
+    elif q_out is not None:
+        raise ValueError("q_out without q")
+    for name, o, like in (("q_out", q_out, q), ("k_out", k_out, k)):
+        if o is not None and o is not like:
+            _type_of(name, o, (k.dtype,))
+            _heads(name, o)
+            if o.shape != like.shape:
+                raise ValueError(f"{name} must be {tuple(like.shape)}, got {tuple(o.shape)}")
+    if k_out is not None and k_out.data_ptr() == k.data_ptr() and t > 0:
+        raise ValueError("k_out must not be k: the keys are still read while it is written")
+    dev = k.device
+    _same_device(dev, v=v, slot_mapping=slot_mapping, k_cache=k_cache, v_cache=v_cache, k_scale=k_scale, v_scale=v_scale,
+                 positions=positions, inv_freq=inv_freq, q=q, q_out=q_out, k_out=k_out)
+
+    def ptr(x):
+        return None if x is None else x.data_ptr()
+
+    def strides(x):
+        return (0, 0) if x is None else (x.stride(0), x.stride(1))
+    with _on(dev):
+        _l.check(_l.load_library().ucmr_kv_append(
+            k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0), v.stride(1), t, hkv, d, dt,
+            slot_mapping.data_ptr(), slot_mapping.dtype == torch.int64, k_cache.data_ptr(), *k_cache.stride()[:3],
+            v_cache.data_ptr(), *v_cache.stride()[:3], k_cache.shape[0], k_cache.shape[1], kind, ptr(k_scale), ptr(v_scale),
+            ptr(positions), positions is not None and positions.dtype == torch.int64, ptr(inv_freq), rot,
+            bool(interleaved), float(mscale), ptr(q), hq, *strides(q), ptr(q_out), *strides(q_out), ptr(k_out),
+            *strides(k_out), _raw_stream(dev)), "ucmr_kv_append")
+    return q_out
+
+
+def paged_attention_workspace_bytes(head_dim: int) -> int:
+    return int(_l.load_library().ucmr_paged_attention_workspace_bytes(int(head_dim)))
+
+
+def new_attention_workspace(head_dim: int, device) -> torch.Tensor:
+    """Workspace for ``paged_attention``, cleared; one per stream that may run beside others."""
+    return torch.zeros(paged_attention_workspace_bytes(head_dim), dtype=torch.uint8, device=device)
+
+
+def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, block_table: torch.Tensor,
+                    seq_lens: torch.Tensor, *, k_scale: Optional[torch.Tensor] = None,
+                    v_scale: Optional[torch.Tensor] = None, query_start: Optional[torch.Tensor] = None,
+                    max_query_len: Optional[int] = None, scale: Optional[float] = None, causal: bool = True,
+                    out: Optional[torch.Tensor] = None, want_lse: bool = False, lse: Optional[torch.Tensor] = None,
+                    workspace: Optional[torch.Tensor] = None):
+    """Attention of q [T, Hq, D] over the paged caches [NB, BS, Hkv, D]; see ``ucmr_paged_attention``.
+
+    ``block_table`` int32 [B, max_blocks], or [B, Hkv, max_blocks] for blocks chosen per kv head, and ``seq_lens`` int32
+    [B] - a request's own, or ``Retrieval.physical`` and ``Retrieval.new_seq_lens`` (with the last block among the
+    chosen).  One query token per request (T = B), or request b's tokens at query_start[b] .. query_start[b+1] with
+    ``max_query_len`` at least the largest count.  ``scale`` defaults to 1 / sqrt(D).  Returns out, or (out, lse) when the
+    log-sum-exp (float32 [T, Hq]) is wanted.  Rows outside every request are left as they were."""
+    dt = _type_of("q", q, _ACTIVATIONS)
+    _heads("q", q)
+    t, hq, d = q.shape
+    if not isinstance(k_cache, torch.Tensor) or k_cache.dim() != 4:
+        raise ValueError("k_cache must be [NB, BS, Hkv, D]")
+    nb, bs, hkv, _ = k_cache.shape
+    kind = _check_cache(k_cache, v_cache, k_scale, v_scale, q.dtype, hkv, d)
+    if hkv == 0 or hq == 0 or hq % hkv:
+        raise ValueError("number of query heads must be a multiple of the kv heads")
+    _need_cuda("block_table", block_table, torch.int32, contiguous=False)
+    if block_table.dim() not in (2, 3) or (block_table.stride(-1) != 1 and block_table.shape[-1] > 1):
+        raise ValueError("block_table must be [B, max_blocks] or [B, Hkv, max_blocks] with a unit inner stride")
+    b, mb = block_table.shape[0], block_table.shape[-1]
+    if block_table.dim() == 3 and block_table.shape[1] not in (1, hkv):
+        raise ValueError(f"a per-head block_table must be [B, {hkv}, max_blocks], got {tuple(block_table.shape)}")
+    bt_h = block_table.stride(1) if block_table.dim() == 3 and block_table.shape[1] > 1 else 0
+    _need_cuda("seq_lens", seq_lens, torch.int32)
+    if seq_lens.shape != (b,):
+        raise ValueError(f"seq_lens must be [{b}], got {tuple(seq_lens.shape)}")
+    if query_start is None:
+        if t != b:
+            raise ValueError(f"{t} query tokens for {b} requests: give query_start and max_query_len")
+        max_query_len = 1
+    else:
+        _need_cuda("query_start", query_start, torch.int32)
+        if query_start.shape != (b + 1,):
+            raise ValueError(f"query_start must be [{b + 1}], got {tuple(query_start.shape)}")
+        if max_query_len is None or max_query_len < 0:
+            raise ValueError("query_start needs max_query_len, the largest number of query tokens of a request")
+    if out is None:
+        out = torch.empty((t, hq, d), dtype=q.dtype, device=q.device)
+    else:
+        if _type_of("out", out, (q.dtype,)) != dt or out.shape != q.shape:
+            raise ValueError(f"out must be like q: {tuple(q.shape)}, got {tuple(out.shape)}")
+        _heads("out", out)
+    if lse is not None:
+        want_lse = True
+        _need_cuda("lse", lse, torch.float32)
+        if lse.shape != (t, hq):
+            raise ValueError(f"lse must be [{t}, {hq}], got {tuple(lse.shape)}")
+    elif want_lse:
+        lse = torch.empty((t, hq), dtype=torch.float32, device=q.device)
+    dev = q.device
+    if workspace is None:
+        workspace = new_attention_workspace(d, dev)
+    else:
+        _need_cuda("workspace", workspace)
+    _same_device(dev, k_cache=k_cache, v_cache=v_cache, k_scale=k_scale, v_scale=v_scale, block_table=block_table,
+                 seq_lens=seq_lens, query_start=query_start, out=out, lse=lse, workspace=workspace)
+    with _on(dev):
+        _l.check(_l.load_library().ucmr_paged_attention(
+            q.data_ptr(), t, hq, d, q.stride(0), q.stride(1), dt, k_cache.data_ptr(), *k_cache.stride()[:3],
+            v_cache.data_ptr(), *v_cache.stride()[:3], nb, bs, hkv, kind, None if k_scale is None else k_scale.data_ptr(),
+            None if v_scale is None else v_scale.data_ptr(), block_table.data_ptr(), mb, block_table.stride(0), bt_h,
+            seq_lens.data_ptr(), None if query_start is None else query_start.data_ptr(), int(max_query_len), b,
+            float(d ** -0.5 if scale is None else scale), bool(causal), out.data_ptr(), out.stride(0), out.stride(1),
+            None if lse is None else lse.data_ptr(), workspace.data_ptr(), workspace.numel() * workspace.element_size(),
+            _raw_stream(dev)), "ucmr_paged_attention")
+    return (out, lse) if want_lse else out
