@@ -13,7 +13,7 @@ CSRC = os.path.join(PKG_DIR, "csrc")
 INCLUDE = os.path.join(os.path.dirname(PKG_DIR), "include")
 LIB_PATH = os.path.join(PKG_DIR, "libucmr_b200.so")
 SOURCES = ["api.cu", "scan.cu", "scan_ring.cu", "scan_rows.cu", "topk.cu", "gather.cu", "encode.cu", "noalloc.cu", "float_retrieval.cu",
-           "rotary.cu", "kv_append.cu", "paged_attention.cu"]
+           "rotary.cu", "kv_append.cu", "paged_attention.cu", "paged_prefill.cu"]
 HEADERS = ["common.cuh", "rotary.cuh", "paged_attention.cuh"]
 
 

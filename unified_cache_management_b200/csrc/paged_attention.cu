@@ -31,6 +31,7 @@
 namespace ucmr {
 
 int device_sms();
+int attention_tiles(const AttnParams& p, int D, int dtype, int cache_dtype, cudaStream_t st);  // paged_prefill.cu
 
 enum { kBf16 = 0, kF16 = 1, kE4m3 = 2 };
 
@@ -297,7 +298,7 @@ __global__ void __launch_bounds__(kDecWarps * 32) decode_kernel(const __grid_con
         auto token_of = [&](int i) { return (s.first + i) * kDecUnit + warp * 16 + (lane & 15); };
         auto block_of = [&](int i) {
             const int tok = token_of(i);
-            return i < n_tiles && tok < max_limit ? table[tok / p.BS] : -1;
+            return i < n_tiles && tok < max_limit ? table[p.by_block.div(tok)] : -1;
         };
         auto issue = [&](int i, int blk) {
             const uint32_t stage = ring + (uint32_t)(i % STAGES) * Sh::kStage;
@@ -305,7 +306,7 @@ __global__ void __launch_bounds__(kDecWarps * 32) decode_kernel(const __grid_con
             const bool in = i < n_tiles && tok < max_limit;
             bool live = in && blk >= 0 && blk < p.NB;
             if (in && !live) flag_status(p.status, UCMR_DEV_BAD_BLOCK_ID);
-            const int row = tok - tok / p.BS * p.BS;
+            const int row = tok - p.by_block.div(tok) * p.BS;
             const int64_t ko = live ? blk * p.cs_b[0] + row * p.cs_t[0] + s.h * p.cs_h[0] : 0;
             const int64_t vo = live ? blk * p.cs_b[1] + row * p.cs_t[1] + s.h * p.cs_h[1] : 0;
             const uint32_t mask = __ballot_sync(0xffffffffu, live) & 0xffffu;
@@ -738,7 +739,7 @@ extern "C" int ucmr_paged_attention(const void* q, int64_t T, int Hq, int D, int
     p.cache[0] = k_cache; p.cs_b[0] = kc_stride_block * es; p.cs_t[0] = kc_stride_t * es; p.cs_h[0] = kc_stride_h * es;
     p.cache[1] = v_cache; p.cs_b[1] = vc_stride_block * es; p.cs_t[1] = vc_stride_t * es; p.cs_h[1] = vc_stride_h * es;
     p.scale[0] = k_scale; p.scale[1] = v_scale;
-    p.NB = NB; p.BS = BS; p.Hkv = Hkv; p.Hq = Hq; p.G = Hq / Hkv;
+    p.NB = NB; p.BS = BS; p.Hkv = Hkv; p.Hq = Hq; p.G = Hq / Hkv; p.by_block = FastDiv((uint32_t)BS);
     p.table = block_table; p.bt_b = bt_stride_b; p.bt_h = bt_stride_h; p.max_blocks = max_blocks;
     p.seq_lens = seq_lens; p.query_start = query_start; p.T = T; p.B = B;
     p.scale_log2 = scale * 1.4426950408889634f; p.causal = causal;
@@ -748,6 +749,7 @@ extern "C" int ucmr_paged_attention(const void* q, int64_t T, int Hq, int D, int
     p.partial = reinterpret_cast<float*>(static_cast<char*>(workspace) + UCMR_WORKSPACE_HEADER_BYTES + kAttnCounterBytes);
     const int64_t rows = (int64_t)(query_start ? max_query_len : 1) * p.G;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
+    if (rows > 16) return attention_tiles(p, D, dtype, cache_dtype, st);
     switch (D) {
         case 64: return launch_types<64>(p, dtype, cache_dtype, rows, st);
         default: return launch_types<128>(p, dtype, cache_dtype, rows, st);

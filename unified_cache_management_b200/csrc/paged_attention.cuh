@@ -11,12 +11,29 @@ namespace ucmr {
 // Workspace: header (device status word first), one arrival counter per CTA, then two partial results per CTA.
 constexpr int kAttnMaxCtas = 512;
 constexpr int kAttnMaxRows = 16;   // query rows of a partial result
+constexpr int kTileMaxCtas = 160;  // the kernel for many rows: one CTA per SM, 128 rows per partial result
 constexpr size_t kAttnCounterBytes = kAttnMaxCtas * sizeof(int32_t);
 
 inline size_t attn_workspace_bytes(int D)
 {
-    return UCMR_WORKSPACE_HEADER_BYTES + kAttnCounterBytes + (size_t)kAttnMaxCtas * 2 * kAttnMaxRows * (D + 2) * sizeof(float);
+    constexpr size_t few = (size_t)kAttnMaxCtas * 2 * kAttnMaxRows, many = (size_t)kTileMaxCtas * 2 * 128;
+    return UCMR_WORKSPACE_HEADER_BYTES + kAttnCounterBytes + (few > many ? few : many) * (D + 2) * sizeof(float);
 }
+
+// Quotients by a fixed divisor (1 .. 2^31 - 1) for numbers below 2^31, without a division: n / d = (hi(m n) + n) >> l with
+// l = ceil(log2 d), m = floor(2^32 (2^l - d) / d) + 1.
+struct FastDiv {
+    uint32_t m, l;
+    explicit FastDiv(uint32_t d = 1)
+    {
+        l = 0;
+        while (l < 31 && (1u << l) < d) ++l;
+        m = (uint32_t)((((1ull << l) - d) << 32) / d + 1);
+    }
+#ifdef __CUDACC__
+    __device__ __forceinline__ int div(int n) const { return (int)((__umulhi(m, (uint32_t)n) + (uint32_t)n) >> l); }
+#endif
+};
 
 struct AttnParams {
     const void* q;           // [T, Hq, D]
@@ -26,6 +43,7 @@ struct AttnParams {
     const float* scale[2];   // [NB, Hkv], null for a 16-bit cache
     int64_t NB;
     int BS, Hkv, Hq, G;
+    FastDiv by_block;        // division by BS
     const int32_t* table;    // [B, max_blocks] or [B, Hkv, max_blocks]
     int64_t bt_b, bt_h;
     int max_blocks;
