@@ -628,26 +628,7 @@ __global__ void __launch_bounds__(kDecWarps * 32) decode_kernel(const __grid_con
             __syncthreads();
             if (sm.last) {
                 __threadfence();
-                for (int i = tid; i < R * D / 4; i += kDecWarps * 32) {
-                    const int row = i / (D / 4), d = (i - row * (D / 4)) * 4;
-                    if (row0 + row >= n_rows) continue;
-                    auto slot = [&](int c) { return p.partial + ((int64_t)c * 2 + (c == c0 ? 1 : 0)) * kAttnMaxRows * kRowFloats; };
-                    float top = -inf;
-                    for (int c = c0; c <= c1; ++c) top = fmaxf(top, __ldcg(slot(c) + kAttnMaxRows * D + row));
-                    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-                    float sum = 0.f;
-#pragma unroll 4
-                    for (int c = c0; c <= c1; ++c) {
-                        const float* sl = slot(c);
-                        const float mc = __ldcg(sl + kAttnMaxRows * D + row), lc = __ldcg(sl + kAttnMaxRows * (D + 1) + row);
-                        const float4 x = __ldcg(reinterpret_cast<const float4*>(sl + row * D + d));
-                        if (mc == -inf) { sum += lc; continue; }
-                        const float f = exp2_fast(mc - top);
-                        sum += f * lc;
-                        v.x += f * x.x; v.y += f * x.y; v.z += f * x.z; v.w += f * x.w;
-                    }
-                    write_row(row, d, v, sum, top);
-                }
+                attn_join<D, kAttnMaxRows, kDecWarps, QT>(p, c0, c1, s.r.q0, s.h, row0, min(R, n_rows - row0), warp, lane);
             }
         }
         __syncthreads();  // the shared rows are used again
@@ -739,7 +720,7 @@ extern "C" int ucmr_paged_attention(const void* q, int64_t T, int Hq, int D, int
     p.cache[0] = k_cache; p.cs_b[0] = kc_stride_block * es; p.cs_t[0] = kc_stride_t * es; p.cs_h[0] = kc_stride_h * es;
     p.cache[1] = v_cache; p.cs_b[1] = vc_stride_block * es; p.cs_t[1] = vc_stride_t * es; p.cs_h[1] = vc_stride_h * es;
     p.scale[0] = k_scale; p.scale[1] = v_scale;
-    p.NB = NB; p.BS = BS; p.Hkv = Hkv; p.Hq = Hq; p.G = Hq / Hkv; p.by_block = FastDiv((uint32_t)BS);
+    p.NB = NB; p.BS = BS; p.Hkv = Hkv; p.Hq = Hq; p.G = Hq / Hkv; p.by_block = FastDiv::by((uint32_t)BS);
     p.table = block_table; p.bt_b = bt_stride_b; p.bt_h = bt_stride_h; p.max_blocks = max_blocks;
     p.seq_lens = seq_lens; p.query_start = query_start; p.T = T; p.B = B;
     p.scale_log2 = scale * 1.4426950408889634f; p.causal = causal;

@@ -24,11 +24,11 @@ inline size_t attn_workspace_bytes(int D)
 // l = ceil(log2 d), m = floor(2^32 (2^l - d) / d) + 1.
 struct FastDiv {
     uint32_t m, l;
-    explicit FastDiv(uint32_t d = 1)
+    static FastDiv by(uint32_t d)
     {
-        l = 0;
+        uint32_t l = 0;
         while (l < 31 && (1u << l) < d) ++l;
-        m = (uint32_t)((((1ull << l) - d) << 32) / d + 1);
+        return FastDiv{(uint32_t)((((1ull << l) - d) << 32) / d + 1), l};
     }
 #ifdef __CUDACC__
     __device__ __forceinline__ int div(int n) const { return (int)((__umulhi(m, (uint32_t)n) + (uint32_t)n) >> l); }
@@ -92,6 +92,90 @@ __device__ __forceinline__ float exp2_fast(float x)
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
+}
+
+template <typename T> struct Out16;
+template <> struct Out16<__nv_bfloat16> {
+    static __device__ __forceinline__ uint32_t pack(float a, float b)
+    {
+        const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+        return reinterpret_cast<const uint32_t&>(h);
+    }
+};
+template <> struct Out16<__half> {
+    static __device__ __forceinline__ uint32_t pack(float a, float b)
+    {
+        const __half2 h = __floats2half2_rn(a, b);
+        return reinterpret_cast<const uint32_t&>(h);
+    }
+};
+
+// Adds up the partial results of one item's CTAs c0 .. c1, in this order, and writes its `rows` rows (from row0 of the
+// request).  CTA c's part lies in slot 2 c, or 2 c + 1 for c0, whose part is the last of its stretch; a slot holds SLOT_ROWS
+// rows of D unnormalised values, then their references, then their sums.  One warp per row: the lanes hold the parts'
+// weights, then D / 32 columns each; eight parts are on their way at a time.
+template <int D, int SLOT_ROWS, int WARPS, typename QT>
+__device__ __forceinline__ void attn_join(const AttnParams& p, int c0, int c1, int q0, int h, int row0, int rows, int warp, int lane)
+{
+    constexpr int W = D / 32;
+    const float inf = __uint_as_float(0x7f800000u);
+    auto slot = [&](int c) { return p.partial + ((int64_t)c * 2 + (c == c0 ? 1 : 0)) * SLOT_ROWS * (D + 2); };
+#pragma unroll 1
+    for (int r = warp; r < rows; r += WARPS) {
+        float top = -inf;
+#pragma unroll 1
+        for (int c = c0 + lane; c <= c1; c += 32) top = fmaxf(top, __ldcg(slot(c) + SLOT_ROWS * D + r));
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+        float v[W], sum = 0.f;
+#pragma unroll
+        for (int i = 0; i < W; ++i) v[i] = 0.f;
+#pragma unroll 1
+        for (int first = c0; first <= c1; first += 32) {
+            const int c = first + lane;
+            float weight = 0.f;
+            if (c <= c1) {
+                const float m = __ldcg(slot(c) + SLOT_ROWS * D + r), l = __ldcg(slot(c) + SLOT_ROWS * (D + 1) + r);
+                weight = m == -inf ? 0.f : exp2_fast(m - top);
+                sum += m == -inf ? l : weight * l;   // (a sum that is NaN stays one)
+            }
+            const int here = min(32, c1 - first + 1);
+#pragma unroll 1
+            for (int k = 0; k < here; k += 8) {
+                float x[8][W], f[8];
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    f[j] = __shfl_sync(0xffffffffu, weight, (k + j) & 31);
+                    if (k + j >= here) f[j] = 0.f;
+                    const float* at = slot(min(first + k + j, c1)) + r * D + lane * W;
+                    if constexpr (W == 4) {
+                        const float4 y = __ldcg(reinterpret_cast<const float4*>(at));
+                        x[j][0] = y.x; x[j][1] = y.y; x[j][2] = y.z; x[j][3] = y.w;
+                    } else {
+                        const float2 y = __ldcg(reinterpret_cast<const float2*>(at));
+                        x[j][0] = y.x; x[j][1] = y.y;
+                    }
+                }
+#pragma unroll
+                for (int j = 0; j < 8; ++j)
+                    if (f[j] != 0.f)
+#pragma unroll
+                        for (int i = 0; i < W; ++i) v[i] += f[j] * x[j][i];
+            }
+        }
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+        const float inv = sum == 0.f ? 0.f : 1.f / sum;
+        const int gr = row0 + r;
+        const int64_t tok = q0 + gr / p.G;
+        const int head = h * p.G + gr % p.G;
+        QT* out = static_cast<QT*>(p.out) + tok * p.os_t + (int64_t)head * p.os_h + lane * W;
+        if constexpr (W == 4)
+            *reinterpret_cast<uint2*>(out) = make_uint2(Out16<QT>::pack(v[0] * inv, v[1] * inv), Out16<QT>::pack(v[2] * inv, v[3] * inv));
+        else
+            *reinterpret_cast<uint32_t*>(out) = Out16<QT>::pack(v[0] * inv, v[1] * inv);
+        if (lane == 0 && p.lse != nullptr) p.lse[tok * p.Hq + head] = sum == 0.f ? -inf : (top + log2f(sum)) * 0.69314718055994531f;
+    }
 }
 
 #endif

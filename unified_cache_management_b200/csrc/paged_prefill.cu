@@ -10,8 +10,10 @@
 //                    (128-byte swizzle), e4m3 codes converted to fp16 on the way
 //   warp 16          TMEM; one thread issues the products
 //   warp 17          one thread works out the CTA's segments
-//   warp 18          plans the token tiles: block table, row offsets, scales (warp 19 only completes the warpgroup)
-// Registers are dealt out accordingly: 112 for a softmax thread, 88 for a loader's, 80 for the others.
+//   warps 18, 19     plan the token tiles ahead of the loaders: block table, row offsets, rows on their way into L2; scales
+// Registers are dealt out accordingly: 112 for a softmax thread, 88 for a loader's, 80 for the others.  Between them the
+// roles' loops have to stay in the SM's instruction cache (with twice the unrolling every role ran at half its speed):
+// hence short loops where straight runs would do.
 // Two chains keep the tensor core busy while a softmax runs.  Their steps alternate; within a chain, P V of a token tile
 // and Q K^T of the chain's next one are issued back to back.
 //   "dual" item: more than 128 rows, the chains are rows 0-127 and 128-255 and share every token tile;
@@ -37,7 +39,7 @@ namespace tile {
 enum { kBf16 = 0, kF16 = 1, kE4m3 = 2 };
 
 constexpr int kTok = 128;            // tokens per tile
-constexpr int kThreads = 640;         // four warpgroups at work, and one whose first warp issues the products
+constexpr int kThreads = 640;         // five warpgroups
 constexpr int kWarps = kThreads / 32;
 constexpr int kLoaders = 128;         // for the keys, and as many for the values
 constexpr int kStages = 2;           // of keys and of values each
@@ -55,71 +57,36 @@ template <int D> struct Sizes {
 };
 
 struct Meta {
-    float ks[kTok], vs[kTok];        // scales per token, for a tile whose scales do not come down to one
+    float tok[2][kTok];              // scales per token, keys and values, for a tile whose scales do not come down to one
     uint32_t valid[4];
-    float kscale, vscale;            // scale of the whole tile
-    int kgeneral, vgeneral;          // ks, vs are in use instead
+    float scale[2];                  // scale of the whole tile
+    int general[2];                  // the scales per token are in use instead
+    int bad;                         // tokens before the end are missing
 };
 
-// One scale for a tile, from the scales of its 128 tokens (four per lane).  All alike: that one.  Powers of two within 2^15
-// of one another: the largest, and the codes are multiplied by the quotient on the way to fp16 - exactly, since a code is a
-// multiple of 2^-9 and fp16 holds multiples of 2^-24.  Otherwise the softmax takes the scales token by token.
-struct TileScale {
-    float scale;
-    bool none, fold, general;   // none: no scale but 0
-    __device__ __forceinline__ TileScale(const float (&s)[4], const bool (&live)[4])
-    {
-        uint32_t lo = 0xffffffffu, hi = 0, odd = 0;
-        bool zero = false;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const uint32_t b = __float_as_uint(s[i]);
-            if (!live[i]) continue;
-            if (b == 0) { zero = true; continue; }
-            lo = min(lo, b);
-            hi = max(hi, b);
-            odd |= (b & 0x807fffffu) | (b >= 0x7f800000u ? 1u : 0u);   // no power of two, negative, subnormal
-        }
-        lo = __reduce_min_sync(0xffffffffu, lo);
-        hi = __reduce_max_sync(0xffffffffu, hi);
-        none = hi == 0;
-        const bool same = none || (lo == hi && !__any_sync(0xffffffffu, zero));
-        fold = general = false;
-        if (!same) {
-            const bool near = !__any_sync(0xffffffffu, odd != 0) && (hi >> 23) - (lo >> 23) <= 15;
-            fold = near;
-            general = !near;
-        }
-        scale = none ? 0.f : __uint_as_float(hi);
-    }
-    // s / scale as two fp16 values: 1 unless the tile folds, else 2^-d with d up to 15 (the last one subnormal), 0 for 0
-    __device__ __forceinline__ uint32_t quotient(float s) const
-    {
-        if (!fold) return 0x3c003c00u;
-        if (s == 0.f) return 0;
-        const uint32_t d = (__float_as_uint(scale) >> 23) - (__float_as_uint(s) >> 23);
-        return (d < 15 ? (15 - d) << 10 : 0x200u) * 0x10001u;
-    }
-};
-
-__device__ __forceinline__ uint4 load_if(const unsigned char* p, bool on)
+// Sixteen bytes if `on`, zeros otherwise; `swap`: the two halves in the other order.
+__device__ __forceinline__ uint4 load_if(const unsigned char* p, bool on, bool swap)
 {
     uint4 v;
     asm volatile(
         "{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %5, 0;\n\t"
         "mov.b32 %0, 0;\n\tmov.b32 %1, 0;\n\tmov.b32 %2, 0;\n\tmov.b32 %3, 0;\n\t"
-        "@q ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];\n\t}"
+        "@q ld.global.nc.L1::no_allocate.v2.u32 {%0, %1}, [%4];\n\t"
+        "@q ld.global.nc.L1::no_allocate.v2.u32 {%2, %3}, [%6];\n\t}"
         : "=&r"(v.x), "=&r"(v.y), "=&r"(v.z), "=&r"(v.w)
-        : "l"(p), "r"((uint32_t)on));
+        : "l"(p + (swap ? 8 : 0)), "r"((uint32_t)on), "l"(p + (swap ? 0 : 8)));
     return v;
 }
 
 // What the loaders have to know of a token tile.
 struct TileSlot {
     int64_t off[2][kTok];            // byte offsets of the tokens' rows, keys and values; -1 = nothing there
+    int block[kTok];                 // their blocks; -1 = nothing there
+    int head, bad;                   // kv head; tokens before the end are missing
     uint32_t fold[2][kTok];          // a token's scale over its tile's, twice in fp16
     int edge;                        // first token if some of the item's rows see the tile's tokens and some do not, else kNoEdge
     int seen;                        // tokens that all rows see
+    int folds[2];                    // the quotients are in use
     int end;                         // no tile: the last slot
 };
 constexpr int kNoEdge = 0x7fffffff;
@@ -133,6 +100,7 @@ struct Segment {
     int len, nq;
     int min_limit, max_limit;   // fewest and most tokens that one of the item's rows sees
     int c0, c1;                 // CTAs that share the item
+    int once;                   // no other item reads the same tokens: they are not in L2 yet
 };
 
 template <int D>
@@ -142,10 +110,12 @@ struct Shared {
     alignas(1024) unsigned char v[kStages][Sizes<D>::kTileBytes];
     Meta meta[kMetaSlots];
     TileSlot tile[kTileSlots];
+    int entry[2][kTok];              // block-table entries of the tile to be placed and of the one after
+    float scale[2][2][kTok];         // scales of the tile to be settled and of the one after
     float merge_m[128], merge_l[128];
     alignas(8) uint64_t k_full[kStages], k_empty[kStages], v_full[kStages], v_empty[kStages];
     uint64_t s_full[2], p_full[2], o_full[2], q_full;
-    uint64_t seg_full[kSegments], seg_empty[kSegments], t_full[kTileSlots], t_empty[kTileSlots];
+    uint64_t seg_full[kSegments], seg_empty[kSegments], t_full[kTileSlots], t_empty[kTileSlots], t_placed[kTileSlots];
     Segment seg[kSegments];
     unsigned long long sums[2][kWarps];
     unsigned long long start_units;
@@ -250,6 +220,12 @@ __device__ __forceinline__ float2 unpair(uint64_t v)
     asm("mov.b64 {%0, %1}, %2;" : "=r"(lo), "=r"(hi) : "l"(v));
     return make_float2(__uint_as_float(lo), __uint_as_float(hi));
 }
+__device__ __forceinline__ float max3(float a, float b, float c)
+{
+    float d;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
 __device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c)
 {
     uint64_t d;
@@ -272,19 +248,33 @@ __device__ __forceinline__ void st16(uint32_t addr, const uint32_t (&r)[16])
         : "memory");
 }
 
-// Bounded wait; after a time-out, here or in another role, nothing waits any more.
+// Bounded waits: a number of tries, each of which the hardware may stretch from some 20 ns to a microsecond or so (a tenth of
+// a second to a few seconds in all) - no clock is read, since these few instructions stand in every loop of every role, and
+// the roles share the instruction cache.
+constexpr uint32_t kTries = 1u << 22;
+
+// After a time-out, here or in another role, nothing waits any more.
 template <int D>
 __device__ __forceinline__ void wait(Shared<D>& sm, uint64_t* bar, uint32_t parity, int32_t* status)
 {
-    if (mbar_try_wait(bar, parity)) return;
-    const unsigned long long t0 = global_timer_ns();
-    for (;;) {
 #pragma unroll 1
-        for (uint32_t i = 0; i < 256; ++i) {
-            if (mbar_try_wait(bar, parity)) return;
-            if (sm.abort) return;
+    for (uint32_t n = 0; !mbar_try_wait(bar, parity); ++n) {
+        if (sm.abort) return;
+        if (n > kTries) {
+            sm.abort = 1;
+            flag_status(status, UCMR_DEV_WAIT_TIMEOUT);
         }
-        if (global_timer_ns() - t0 > kWaitLimitNs) {
+    }
+}
+
+// Wait in the rings of segments and planned tiles, which keep turning when the rest has given up: the abort flag does not
+// end it, so that no role reads what another has not finished with.
+template <int D>
+__device__ __forceinline__ void wait_ring(Shared<D>& sm, uint64_t* bar, uint32_t parity, int32_t* status)
+{
+#pragma unroll 1
+    for (uint32_t n = 0; !mbar_try_wait(bar, parity); ++n) {
+        if (n > 8 * kTries) {
             sm.abort = 1;
             flag_status(status, UCMR_DEV_WAIT_TIMEOUT);
             return;
@@ -292,20 +282,9 @@ __device__ __forceinline__ void wait(Shared<D>& sm, uint64_t* bar, uint32_t pari
     }
 }
 
-// Wait in the ring of segments, which keeps turning when the rest has given up: the abort flag does not end it, so that no
-// role reads a segment that another has not finished with.
-template <int D>
-__device__ __forceinline__ void wait_ring(Shared<D>& sm, uint64_t* bar, uint32_t parity, int32_t* status)
+__device__ __forceinline__ void copy4(void* dst, const void* src)
 {
-    if (mbar_try_wait(bar, parity)) return;
-    const unsigned long long t0 = global_timer_ns();
-    while (!mbar_try_wait(bar, parity)) {
-        if (global_timer_ns() - t0 > 8 * kWaitLimitNs) {
-            sm.abort = 1;
-            flag_status(status, UCMR_DEV_WAIT_TIMEOUT);
-            return;
-        }
-    }
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_u32(dst)), "l"(src) : "memory");
 }
 
 __device__ __forceinline__ void bar_sync(int id, int threads) { asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory"); }
@@ -400,6 +379,7 @@ struct SegmentWalk {
             s.n_rows = r.nq * p.G;
             s.row0 = rt * line.rows;
             const int last_row = min(s.n_rows, s.row0 + line.rows) - 1;
+            s.once = tiles == 1;
             s.dual = last_row - s.row0 >= 128;
             s.min_limit = attn_limit(p, r, s.row0 / p.G);
             s.max_limit = attn_limit(p, r, last_row / p.G);
@@ -423,12 +403,12 @@ __global__ void __launch_bounds__(kThreads, 1) tile_kernel(const __grid_constant
     // ---- set-up: barriers, TMEM, the CTA's stretch of the line -------------------------------------------------------
     if (tid == 0) {
         for (int i = 0; i < kStages; ++i) {
-            mbar_init(&sm.k_full[i], 4); mbar_init(&sm.k_empty[i], 1);
-            mbar_init(&sm.v_full[i], 4); mbar_init(&sm.v_empty[i], 1);
+            mbar_init(&sm.k_full[i], kLoaders / 32); mbar_init(&sm.k_empty[i], 1);
+            mbar_init(&sm.v_full[i], kLoaders / 32); mbar_init(&sm.v_empty[i], 1);
         }
         for (int i = 0; i < 2; ++i) { mbar_init(&sm.s_full[i], 1); mbar_init(&sm.p_full[i], 4); mbar_init(&sm.o_full[i], 1); }
         for (int i = 0; i < kSegments; ++i) { mbar_init(&sm.seg_full[i], 1); mbar_init(&sm.seg_empty[i], kSegmentReaders); }
-        for (int i = 0; i < kTileSlots; ++i) { mbar_init(&sm.t_full[i], 1); mbar_init(&sm.t_empty[i], 8); }
+        for (int i = 0; i < kTileSlots; ++i) { mbar_init(&sm.t_full[i], 1); mbar_init(&sm.t_placed[i], 1); mbar_init(&sm.t_empty[i], 2 * kLoaders / 32); }
         mbar_init(&sm.q_full, 8);
         sm.abort = 0;
         sm.odd = 0;
@@ -527,43 +507,41 @@ __global__ void __launch_bounds__(kThreads, 1) tile_kernel(const __grid_constant
             if (s.n > 0 && (s.dual || T == 0)) {
                 const QT* qr = static_cast<const QT*>(p.q);
                 if (live) qr += (int64_t)(s.q0 + row / p.G) * p.qs_t + (int64_t)(s.h * p.G + row % p.G) * p.qs_h;
+                uint4 v[D / 8];                      // (all loads at once)
+#pragma unroll
+                for (int c = 0; c < D / 8; ++c) {
+                    v[c] = make_uint4(0, 0, 0, 0);
+                    if (live) v[c] = *reinterpret_cast<const uint4*>(qr + c * 8);
+                }
                 float down = 1.f;
                 if constexpr (C == kE4m3) {
-                    uint32_t big = 0;
-                    if (live) {
-#pragma unroll 4
-                        for (int c = 0; c < D / 8; ++c) {
-                            const uint4 v = *reinterpret_cast<const uint4*>(qr + c * 8);
-                            const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+                    uint32_t m2 = 0;                 // largest magnitudes of the even and odd elements, as 16-bit patterns
 #pragma unroll
-                            for (int i = 0; i < 4; ++i) {
-                                const float2 f = unpack2(w[i], kQBf16);
-                                const uint32_t a = __float_as_uint(fabsf(f.x)), b2 = __float_as_uint(fabsf(f.y));
-                                if (a < 0x7f800000u) big = max(big, a);
-                                if (b2 < 0x7f800000u) big = max(big, b2);
-                            }
-                        }
+                    for (int c = 0; c < D / 8; ++c) {
+                        m2 = __vmaxu2(m2, v[c].x & 0x7fff7fffu); m2 = __vmaxu2(m2, v[c].y & 0x7fff7fffu);
+                        m2 = __vmaxu2(m2, v[c].z & 0x7fff7fffu); m2 = __vmaxu2(m2, v[c].w & 0x7fff7fffu);
                     }
+                    const float2 m = unpack2(m2, kQBf16);
+                    uint32_t big = __float_as_uint(fmaxf(m.x, m.y));
+                    if (!(m.x <= 3.402823466e38f && m.y <= 3.402823466e38f)) big = 0;   // (the row is not finite: nor is its result)
                     const int e = big == 0 ? 0 : max(-125, min(125, (int)(big >> 23) - 127));
                     down = __uint_as_float((uint32_t)(127 - e) << 23);
                     if (!s.dual) sm.merge_m[local] = __uint_as_float((uint32_t)(127 + e) << 23);
                     qmul *= __uint_as_float((uint32_t)(127 + e) << 23);
                 }
                 unsigned char* dst = sm.q[s.dual ? T : 0];
-#pragma unroll 4
+#pragma unroll
                 for (int c = 0; c < D / 8; ++c) {
-                    uint4 v = make_uint4(0, 0, 0, 0);
-                    if (live) v = *reinterpret_cast<const uint4*>(qr + c * 8);
                     if constexpr (C == kE4m3) {
-                        uint32_t w[4] = {v.x, v.y, v.z, v.w};
+                        uint32_t w[4] = {v[c].x, v[c].y, v[c].z, v[c].w};
 #pragma unroll
                         for (int i = 0; i < 4; ++i) {
                             const float2 f = unpack2(w[i], kQBf16);
                             w[i] = pack2<kF16>(f.x * down, f.y * down);
                         }
-                        v = make_uint4(w[0], w[1], w[2], w[3]);
+                        v[c] = make_uint4(w[0], w[1], w[2], w[3]);
                     }
-                    *reinterpret_cast<uint4*>(dst + swz(c >> 3, local, c & 7)) = v;
+                    *reinterpret_cast<uint4*>(dst + swz(c >> 3, local, c & 7)) = v[c];
                 }
                 fence_proxy_async();
             }
@@ -580,6 +558,7 @@ __global__ void __launch_bounds__(kThreads, 1) tile_kernel(const __grid_constant
             const int warp_limit = __reduce_min_sync(0xffffffffu, limit);
             float ref = -inf, sum = 0.f;
             int vexp = -200;
+            float vf_of = 0.f, vf_log = 0.f, vf_inv = 1.f;       // a factor on the weights, its logarithm and reciprocal
             for (int st = 0; st < steps; ++st) {
                 const int i = s.dual ? st : 2 * st + T;          // token tile of the segment
                 const int tok0 = (s.first + i) * kTok;
@@ -592,21 +571,21 @@ __global__ void __launch_bounds__(kThreads, 1) tile_kernel(const __grid_constant
                 float vdown = 1.f;
                 bool kgen = false, vgen = false;
                 if constexpr (C == kE4m3) {
-                    const float vscale = mt.vscale;
-                    kgen = mt.kgeneral != 0;
-                    vgen = mt.vgeneral != 0;
+                    const float vscale = mt.scale[1];
+                    kgen = mt.general[0] != 0;
+                    vgen = mt.general[1] != 0;
                     const int e = max(-100, min(128, (int)((__float_as_uint(vscale) & 0x7fffffffu) >> 23) - 126));
                     if (e > vexp) {
                         vdown = vexp == -200 ? 0.f : exp2_fast((float)(vexp - e));
                         vexp = e;
                     }
                     vf = exp2_fast(kShift - (float)vexp);
-                    if (!kgen) kf *= mt.kscale;
+                    if (!kgen) kf *= mt.scale[0];
                     if (!vgen) vf *= vscale;
                 }
-                const bool full = (mt.valid[0] & mt.valid[1] & mt.valid[2] & mt.valid[3]) == 0xffffffffu;
-                // One scale, every token there for every row of the warp.
-                const bool plain = !kgen && !vgen && full && tok0 + kTok <= warp_limit && kf >= 0.f && vf > 0.f;
+                // One scale, and no token missing but at the end: columns from `bound` on are hidden.
+                const bool plain = !kgen && !vgen && kf > 0.f && vf > 0.f && !mt.bad;
+                const int bound = limit - tok0;
                 float alpha = 1.f;
                 auto raise = [&](float top) {
                     if (top > ref + kLazy || (ref == -inf && top > -inf)) {
@@ -628,30 +607,41 @@ __global__ void __launch_bounds__(kThreads, 1) tile_kernel(const __grid_constant
                     }
                 };
                 if (plain) {
-                    // Short loops rather than one run through 128 columns: the roles share the instruction cache.  P of
-                    // columns 32c.. goes to 64 + 16c..; from the last ones down no column is overwritten before it is read.
+                    const bool cut = tok0 + kTok > warp_limit;
+                    uint32_t r[32];
+                    auto fetch = [&](int c) {        // columns 32c ..; hidden ones -> no weight
+                        ld32(tS_at + c * 32, r);
+                        wait_ld();
+                        if (cut) {
+                            const int from = bound - c * 32;
+#pragma unroll
+                            for (int j = 0; j < 32; ++j)
+                                if (j >= from) r[j] = 0xff800000u;
+                        }
+                    };
                     float t4[4] = {-inf, -inf, -inf, -inf};
 #pragma unroll 1
-                    for (int c = 0; c < 2; ++c) {
-                        uint32_t r[2][32];
-                        ld32(tS_at + c * 64, r[0]);
-                        ld32(tS_at + c * 64 + 32, r[1]);
-                        wait_ld();
+                    for (int c = 0; c < 4; ++c) {
+                        fetch(c);
 #pragma unroll
-                        for (int k = 0; k < 2; ++k)
-#pragma unroll
-                            for (int j = 0; j < 32; ++j) t4[j & 3] = fmaxf(t4[j & 3], __uint_as_float(r[k][j]));
+                        for (int j = 0; j < 32; j += 2)
+                            t4[(j >> 1) & 3] = max3(t4[(j >> 1) & 3], __uint_as_float(r[j]), __uint_as_float(r[j + 1]));
                     }
                     raise(fmaxf(fmaxf(t4[0], t4[1]), fmaxf(t4[2], t4[3])) * kf);
-                    // exp2(score - reference) * vf in one exponential; the sum is taken back to weights at the end
-                    const float base = (C == kBf16 ? 0.f : log2f(vf)) - (ref == -inf ? 0.f : ref);
+                    // exp2(score - reference) * vf in one exponential; the sum is taken back to weights at the end.  P of
+                    // columns 32c.. goes to 64 + 16c..: from the last ones down no column is overwritten before it is read.
+                    if (C != kBf16 && vf != vf_of) {
+                        vf_of = vf;
+                        vf_log = log2f(vf);
+                        vf_inv = 1.f / vf;
+                    }
+                    const float base = vf_log - (ref == -inf ? 0.f : ref);
                     const uint64_t kf2 = pairf(kf, kf), base2 = pairf(base, base);
                     uint64_t acc[2] = {0, 0};
 #pragma unroll 1
                     for (int c = 3; c >= 0; --c) {
-                        uint32_t r[32], w[16];
-                        ld32(tS_at + c * 32, r);
-                        wait_ld();
+                        uint32_t w[16];
+                        fetch(c);
 #pragma unroll
                         for (int j = 0; j < 32; j += 2) {
                             const float2 x = unpair(fma2(pair(r[j], r[j + 1]), kf2, base2));
@@ -662,7 +652,7 @@ __global__ void __launch_bounds__(kThreads, 1) tile_kernel(const __grid_constant
                         st16(tS_at + 64 + c * 16, w);
                     }
                     const float2 a = unpair(add2(acc[0], acc[1]));
-                    sum += C == kBf16 ? a.x + a.y : (a.x + a.y) / vf;
+                    sum += (a.x + a.y) * vf_inv;
                 } else {
                     float top = -inf;
 #pragma unroll 1
@@ -674,7 +664,7 @@ __global__ void __launch_bounds__(kThreads, 1) tile_kernel(const __grid_constant
 #pragma unroll
                         for (int j = 0; j < 16; ++j) {
                             float x = __uint_as_float(r[j]) * kf;
-                            if (kgen) x *= mt.ks[c * 16 + j];
+                            if (kgen) x *= mt.tok[0][c * 16 + j];
                             top = tok0 + c * 16 + j < limit && ((seen16 >> j) & 1u) ? fmaxf(top, x) : top;
                         }
                     }
@@ -694,12 +684,12 @@ __global__ void __launch_bounds__(kThreads, 1) tile_kernel(const __grid_constant
 #pragma unroll
                             for (int q = 0; q < 2; ++q) {
                                 x[q] = __uint_as_float(r[j + q]) * kf;
-                                if (kgen) x[q] *= mt.ks[c * 16 + j + q];
+                                if (kgen) x[q] *= mt.tok[0][c * 16 + j + q];
                                 const bool seen = tok0 + c * 16 + j + q < limit && ((seen16 >> (j + q)) & 1u);
                                 x[q] = seen ? exp2_fast(x[q] - base) : 0.f;
                                 sum += x[q];
                                 x[q] *= vf;
-                                if (vgen) x[q] = seen ? x[q] * mt.vs[c * 16 + j + q] : 0.f;
+                                if (vgen) x[q] = seen ? x[q] * mt.tok[1][c * 16 + j + q] : 0.f;
                             }
                             w[j / 2] = pack2<kP>(x[0], x[1]);
                         }
@@ -848,33 +838,7 @@ __global__ void __launch_bounds__(kThreads, 1) tile_kernel(const __grid_constant
                 bar_sync(1, 256);
                 if (sm.last) {
                     __threadfence();
-                    for (int i = tid; i < 128 * D / 4; i += 256) {
-                        const int rr = i / (D / 4), d = (i - rr * (D / 4)) * 4;
-                        const int gr = s.row0 + rr;
-                        if (gr >= s.n_rows) break;
-                        auto slot = [&](int c) { return p.partial + ((int64_t)c * 2 + (c == c0 ? 1 : 0)) * 128 * kRowFloats; };
-                        float m = -inf;
-                        for (int c = c0; c <= c1; ++c) m = fmaxf(m, __ldcg(slot(c) + 128 * D + rr));
-                        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-                        float l = 0.f;
-#pragma unroll 2
-                        for (int c = c0; c <= c1; ++c) {
-                            const float* sl = slot(c);
-                            const float mc = __ldcg(sl + 128 * D + rr), lc = __ldcg(sl + 128 * (D + 1) + rr);
-                            const float4 x = __ldcg(reinterpret_cast<const float4*>(sl + rr * D + d));
-                            if (mc == -inf) { l += lc; continue; }
-                            const float f = exp2_fast(mc - m);
-                            l += f * lc;
-                            v.x += f * x.x; v.y += f * x.y; v.z += f * x.z; v.w += f * x.w;
-                        }
-                        const float iv = l == 0.f ? 0.f : 1.f / l;
-                        constexpr int kO = kQBf16 ? kBf16 : kF16;
-                        const int64_t tk = s.q0 + gr / p.G;
-                        const int hd = s.h * p.G + gr % p.G;
-                        *reinterpret_cast<uint2*>(static_cast<QT*>(p.out) + tk * p.os_t + (int64_t)hd * p.os_h + d) =
-                            make_uint2(pack2<kO>(v.x * iv, v.y * iv), pack2<kO>(v.z * iv, v.w * iv));
-                        if (d == 0 && p.lse != nullptr) p.lse[tk * p.Hq + hd] = l == 0.f ? -inf : (m + log2f(l)) * 0.69314718055994531f;
-                    }
+                    attn_join<D, 128, 8, QT>(p, c0, c1, s.q0, s.h, s.row0, min(128, s.n_rows - s.row0), warp, lane);
                 }
             }
             bar_sync(1, 256);  // the queries and the merged rows have been used
@@ -958,36 +922,42 @@ __global__ void __launch_bounds__(kThreads, 1) tile_kernel(const __grid_constant
                 const int st = done % kStages;
                 const TileSlot& slot = sm.tile[done % kTileSlots];
                 if (has) wait(sm, &empty[st], ((done / kStages) & 1) ^ 1, p.status);
-                unsigned char* dst = ring + st * Sizes<D>::kTileBytes;
+                if (has) {
+                    // rows i * kRows + prow: the swizzle of a row depends on row % 8, which all of a thread's rows share
+                    unsigned char* dst = ring + st * Sizes<D>::kTileBytes;
+                    unsigned char* d0 = dst + swz(piece >> 2, prow, c0 + flip);
+                    unsigned char* d1 = dst + swz(piece >> 2, prow, c0 + 1 - flip);
+                    static_assert(kRows % 8 == 0, "swizzle");
+                    const bool folds = slot.folds[kind] != 0;
 #pragma unroll
-                for (int i = 0; i < kPasses; ++i) {
-                    const int row = i * kRows + prow;
-                    if (has) {
-                        const uint32_t mw = slot.fold[kind][row];
-                        const __half2 m = reinterpret_cast<const __half2&>(mw);
-                        const uint32_t w[4] = {flip ? raw[i].z : raw[i].x, flip ? raw[i].w : raw[i].y,
-                                               flip ? raw[i].x : raw[i].z, flip ? raw[i].y : raw[i].w};
+                    for (int i = 0; i < kPasses; ++i) {
+                        const uint32_t w[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
                         uint32_t f[8];
 #pragma unroll
-                        for (int j = 0; j < 8; ++j) {
-                            f[j] = e4m3x2_to_f16x2(j & 1 ? w[j >> 1] >> 16 : w[j >> 1]);
-                            const __half2 v = __hmul2(reinterpret_cast<const __half2&>(f[j]), m);
-                            f[j] = reinterpret_cast<const uint32_t&>(v);
+                        for (int j = 0; j < 8; ++j) f[j] = e4m3x2_to_f16x2(j & 1 ? w[j >> 1] >> 16 : w[j >> 1]);
+                        if (folds) {
+                            const uint32_t mw = slot.fold[kind][i * kRows + prow];
+#pragma unroll
+                            for (int j = 0; j < 8; ++j) {
+                                const __half2 v = __hmul2(reinterpret_cast<const __half2&>(f[j]), reinterpret_cast<const __half2&>(mw));
+                                f[j] = reinterpret_cast<const uint32_t&>(v);
+                            }
                         }
-                        *reinterpret_cast<uint4*>(dst + swz(piece >> 2, row, c0 + flip)) = make_uint4(f[0], f[1], f[2], f[3]);
-                        *reinterpret_cast<uint4*>(dst + swz(piece >> 2, row, c0 + 1 - flip)) = make_uint4(f[4], f[5], f[6], f[7]);
+                        const uint4 a = make_uint4(f[0], f[1], f[2], f[3]), b = make_uint4(f[4], f[5], f[6], f[7]);
+                        *reinterpret_cast<uint4*>(d0 + i * kRows * 128) = a;
+                        *reinterpret_cast<uint4*>(d1 + i * kRows * 128) = b;
                     }
-                    if (more) {
-                        const int64_t off = next.off[kind][row];
-                        raw[i] = load_if(cache + off + piece * 16, off >= 0);
-                    }
-                }
-                if (has) {
                     if (kind == 1 && slot.edge != kNoEdge) sift(st, slot.edge, slot.seen);
-                    drop_slot(done);
                     arrive(&full[st]);
-                    ++done;
                 }
+                if (more) {
+#pragma unroll
+                    for (int i = 0; i < kPasses; ++i) {
+                        const int64_t off = next.off[kind][i * kRows + prow];
+                        raw[i] = load_if(cache + off + piece * 16, off >= 0, flip != 0);
+                    }
+                }
+                if (has) drop_slot(done++);
                 has = more;
             }
         } else {
@@ -1037,7 +1007,7 @@ __global__ void __launch_bounds__(kThreads, 1) tile_kernel(const __grid_constant
         // ================================= products ===============================================================
         if (warp == 16 && lane == 0) {
         uint32_t tiles = 0;                 // token tiles before this segment
-        uint32_t n_p[2] = {0, 0}, n_q = 0;
+        uint32_t n_p = 0, n_q = 0;          // phases seen (a bit per chain)
         for (;;) {
             const Segment& slot = take_segment();
             const int s_n = slot.n;
@@ -1049,9 +1019,10 @@ __global__ void __launch_bounds__(kThreads, 1) tile_kernel(const __grid_constant
             auto scores = [&](int st) {
                 const int i = dual ? st >> 1 : st, T = st & 1;
                 const uint32_t tile = tiles + i, stage = tile % kStages;
-                wait(sm, &sm.k_full[stage], (tile / kStages) & 1, p.status);
-                fence_proxy_async();
-                fence_after();
+                if (!dual || T == 0) {
+                    wait(sm, &sm.k_full[stage], (tile / kStages) & 1, p.status);
+                    fence_proxy_async();
+                }
                 const uint64_t qa = desc_k_major(smem_u32(sm.q[dual ? T : 0])), ka = desc_k_major(smem_u32(sm.k[stage]));
 #pragma unroll
                 for (int ks = 0; ks < D / 16; ++ks) {
@@ -1070,10 +1041,12 @@ __global__ void __launch_bounds__(kThreads, 1) tile_kernel(const __grid_constant
                 if (st >= 0) {
                     const int i = dual ? st >> 1 : st;
                     const uint32_t tile = tiles + i, stage = tile % kStages;
-                    wait(sm, &sm.v_full[stage], (tile / kStages) & 1, p.status);
-                    wait(sm, &sm.p_full[T], n_p[T] & 1, p.status);
-                    ++n_p[T];
-                    fence_proxy_async();
+                    if (!dual || T == 0) {
+                        wait(sm, &sm.v_full[stage], (tile / kStages) & 1, p.status);
+                        fence_proxy_async();
+                    }
+                    wait(sm, &sm.p_full[T], (n_p >> T) & 1, p.status);
+                    n_p ^= 1u << T;
                     fence_after();
                     const uint64_t va = desc_mn_major(smem_u32(sm.v[stage]));
                     const bool first = dual ? i == 0 : st < 2;
@@ -1088,82 +1061,67 @@ __global__ void __launch_bounds__(kThreads, 1) tile_kernel(const __grid_constant
             tiles += s_n;
         }
         } else if (warp == 18) {
-            // ============================= planner: one token tile at a time, four tokens per lane =========================
+            // ============================= places: one token tile at a time, four tokens per lane ==========================
             uint32_t tile = 0;
             for (bool more = true; more;) {
                 const Segment& s = take_segment();
-                const int n = s.n, first = s.first, low = s.min_limit, high = s.max_limit, h = s.h;
+                const int n = s.n, first = s.first, low = s.min_limit, high = s.max_limit, h = s.h, once = s.once;
                 const int32_t* table = p.table + (int64_t)s.b * p.bt_b + (int64_t)s.h * p.bt_h;
                 __syncwarp();
                 if (lane == 0) drop_segment();
                 else ++n_seg;
                 more = n >= 0;
-                // the blocks of the next tile and the scales of this one were asked for a tile earlier
-                int blk[4], blk1[4];
-                float ks[4], vs[4], ks1[4], vs1[4];
-                auto look_up = [&](int i, int (&to)[4]) {
-#pragma unroll
-                    for (int k = 0; k < 4; ++k) {
-                        const int tok = (first + i) * kTok + k * 32 + lane;
-                        to[k] = tok < high ? table[p.by_block.div(tok)] : -1;
-                        if (tok < high && (to[k] < 0 || to[k] >= p.NB)) { flag_status(p.status, UCMR_DEV_BAD_BLOCK_ID); to[k] = -1; }
-                    }
-                };
-                auto look_at_scales = [&](const int (&of)[4], float (&k4)[4], float (&v4)[4]) {
-#pragma unroll
-                    for (int k = 0; k < 4; ++k) {
-                        k4[k] = v4[k] = 0.f;
-                        if (C == kE4m3 && of[k] >= 0) {
-                            const int64_t at = (int64_t)of[k] * p.Hkv + h;
-                            k4[k] = p.scale[0][at];
-                            v4[k] = p.scale[1][at];
+                // The next tile's entries are copied while this one is placed; a lane reads what it has copied itself.
+                auto look_up = [&](int i, uint32_t t) {
+                    if (i < n) {
+#pragma unroll 1
+                        for (int at = lane; at < kTok; at += 32) {
+                            const int tok = (first + i) * kTok + at;
+                            if (tok < high) copy4(&sm.entry[t & 1][at], table + p.by_block.div(tok));
                         }
                     }
+                    asm volatile("cp.async.commit_group;" ::: "memory");
                 };
-                if (n > 0) {
-                    look_up(0, blk1);
-                    look_at_scales(blk1, ks1, vs1);
-                }
+                look_up(0, tile);
+#pragma unroll 1
                 for (int i = 0; i < max(n, more ? 0 : 1); ++i, ++tile) {
                     TileSlot& slot = sm.tile[tile % kTileSlots];
-                    Meta& mt = sm.meta[tile % kMetaSlots];
-                    bool live[4];
-#pragma unroll
-                    for (int k = 0; k < 4; ++k) { blk[k] = blk1[k]; ks[k] = ks1[k]; vs[k] = vs1[k]; live[k] = blk[k] >= 0; }
-                    if (i + 1 < n) {
-                        look_up(i + 1, blk1);
-                        look_at_scales(blk1, ks1, vs1);
-                    }
+                    look_up(i + 1, tile + 1);
+                    asm volatile("cp.async.wait_group 1;" ::: "memory");
                     wait_ring(sm, &sm.t_empty[tile % kTileSlots], ((tile / kTileSlots) & 1) ^ 1, p.status);
                     if (more) {
-                        uint32_t valid[4];
-#pragma unroll
-                        for (int k = 0; k < 4; ++k) {
-                            const int tok = (first + i) * kTok + k * 32 + lane;
+                        const int tok0 = (first + i) * kTok;
+                        bool missing = false;
+#pragma unroll 1
+                        for (int at = lane; at < kTok; at += 32) {
+                            const int tok = tok0 + at;
+                            int blk = tok < high ? sm.entry[tile & 1][at] : -1;
+                            if (blk < 0 || blk >= p.NB) {
+                                missing |= tok < high;
+                                blk = -1;
+                            }
                             const int row = tok - p.by_block.div(tok) * p.BS;
-                            slot.off[0][k * 32 + lane] = live[k] ? blk[k] * p.cs_b[0] + row * p.cs_t[0] + h * p.cs_h[0] : -1;
-                            slot.off[1][k * 32 + lane] = live[k] ? blk[k] * p.cs_b[1] + row * p.cs_t[1] + h * p.cs_h[1] : -1;
-                            valid[k] = __ballot_sync(0xffffffffu, live[k]);
-                        }
-                        if constexpr (C == kE4m3) {
-                            const TileScale tk(ks, live), tv(vs, live);
+                            const int64_t ko = blk * p.cs_b[0] + row * p.cs_t[0] + h * p.cs_h[0];
+                            const int64_t vo = blk * p.cs_b[1] + row * p.cs_t[1] + h * p.cs_h[1];
+                            slot.block[at] = blk;
+                            slot.off[0][at] = blk >= 0 ? ko : -1;
+                            slot.off[1][at] = blk >= 0 ? vo : -1;
+                            // The row on its way into L2, a few tiles before the loaders ask for it (verification of 4
+                            // tokens: 424 -> 323 us); rows that other items read too are there already.
+                            if (blk >= 0 && once) {
+                                constexpr int kRowBytes = D * (C == kE4m3 ? 1 : 2);
 #pragma unroll
-                            for (int k = 0; k < 4; ++k) {
-                                // (values of scale 0 are zeros: so are their codes)
-                                slot.fold[0][k * 32 + lane] = tk.quotient(ks[k]);
-                                slot.fold[1][k * 32 + lane] = tv.none ? 0u : tv.quotient(vs[k]);
-                                if (tk.general) mt.ks[k * 32 + lane] = ks[k];
-                                if (tv.general) mt.vs[k * 32 + lane] = vs[k];
-                            }
-                            if (lane == 0) {
-                                mt.kscale = tk.scale; mt.kgeneral = tk.general;
-                                mt.vscale = tv.none ? 1.f : tv.scale; mt.vgeneral = tv.general;
+                                for (int l = 0; l < kRowBytes; l += 128) {
+                                    asm volatile("prefetch.global.L2 [%0];" ::"l"(static_cast<const char*>(p.cache[0]) + ko + l));
+                                    asm volatile("prefetch.global.L2 [%0];" ::"l"(static_cast<const char*>(p.cache[1]) + vo + l));
+                                }
                             }
                         }
+                        if (missing) flag_status(p.status, UCMR_DEV_BAD_BLOCK_ID);
+                        missing = __any_sync(0xffffffffu, missing);
                         if (lane == 0) {
-#pragma unroll
-                            for (int k = 0; k < 4; ++k) mt.valid[k] = valid[k];
-                            const int tok0 = (first + i) * kTok;
+                            slot.head = h;
+                            slot.bad = missing;
                             slot.edge = tok0 + kTok > low && low < high ? tok0 : kNoEdge;
                             slot.seen = low;
                             slot.end = 0;
@@ -1171,6 +1129,90 @@ __global__ void __launch_bounds__(kThreads, 1) tile_kernel(const __grid_constant
                     } else if (lane == 0) {
                         slot.end = 1;
                     }
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&sm.t_placed[tile % kTileSlots]);
+                }
+            }
+        } else if (warp == 19) {
+            // ============================= scales: asked for when a tile has been placed, used when the next one has ============
+            // One scale for the tile, keys and values each.  All alike: that one.  Powers of two within 2^15 of one another: the
+            // largest, and the codes are multiplied by the quotient on the way to fp16 - exactly, since a code is a multiple
+            // of 2^-9 and fp16 holds multiples of 2^-24.  Otherwise the softmax takes the scales token by token.
+            uint32_t tile = 0;
+#pragma unroll 1
+            for (bool more = true, has = false; more || has; ++tile) {
+                if (more) {
+                    wait_ring(sm, &sm.t_placed[tile % kTileSlots], (tile / kTileSlots) & 1, p.status);
+                    const TileSlot& slot = sm.tile[tile % kTileSlots];
+                    more = !slot.end;
+                    if (C == kE4m3 && more) {
+#pragma unroll 1
+                        for (int at = lane; at < kTok; at += 32) {
+                            const int blk = slot.block[at];
+                            if (blk < 0) continue;
+                            const int64_t from = (int64_t)blk * p.Hkv + slot.head;
+                            copy4(&sm.scale[tile & 1][0][at], p.scale[0] + from);
+                            copy4(&sm.scale[tile & 1][1][at], p.scale[1] + from);
+                        }
+                    }
+                }
+                asm volatile("cp.async.commit_group;" ::: "memory");
+                if (has) {                           // the tile before
+                    asm volatile("cp.async.wait_group 1;" ::: "memory");
+                    const uint32_t t = tile - 1;
+                    TileSlot& slot = sm.tile[t % kTileSlots];
+                    Meta& mt = sm.meta[t % kMetaSlots];
+                    if constexpr (C == kE4m3) {
+#pragma unroll 1
+                        for (int kind = 0; kind < 2; ++kind) {
+                            const float* of = sm.scale[t & 1][kind];
+                            uint32_t lo = 0xffffffffu, hi = 0, odd = 0, zero = 0;
+#pragma unroll 1
+                            for (int at = lane; at < kTok; at += 32) {
+                                if (slot.block[at] < 0) continue;
+                                const uint32_t b = __float_as_uint(of[at]);
+                                if (b == 0) { zero = 1; continue; }
+                                lo = min(lo, b);
+                                hi = max(hi, b);
+                                odd |= (b & 0x807fffffu) | (b >= 0x7f800000u ? 1u : 0u);   // no power of two, negative, subnormal
+                            }
+                            lo = __reduce_min_sync(0xffffffffu, lo);
+                            hi = __reduce_max_sync(0xffffffffu, hi);
+                            const bool none = hi == 0;           // no scale but 0: values are zeros, and so are their codes
+                            int fold = none && kind == 1, general = 0;
+                            if (!none && (lo != hi || __any_sync(0xffffffffu, zero != 0))) {
+                                fold = !__any_sync(0xffffffffu, odd != 0) && (hi >> 23) - (lo >> 23) <= 15;
+                                general = !fold;
+                            }
+                            if (lane == 0) {
+                                mt.scale[kind] = none && kind == 1 ? 1.f : __uint_as_float(hi);
+                                mt.general[kind] = general;
+                                slot.folds[kind] = fold;
+                            }
+                            if (fold || general) {
+#pragma unroll 1
+                                for (int at = lane; at < kTok; at += 32) {
+                                    const float v = slot.block[at] < 0 ? 0.f : of[at];
+                                    // 2^-d with d up to 15 (the last one subnormal), 0 for 0, twice in fp16
+                                    const uint32_t d = (hi >> 23) - (__float_as_uint(v) >> 23);
+                                    slot.fold[kind][at] = v == 0.f ? 0u : (d < 15 ? (15 - d) << 10 : 0x200u) * 0x10001u;
+                                    mt.tok[kind][at] = v;
+                                }
+                            }
+                        }
+                    }
+                    const int bad = slot.bad;
+#pragma unroll 1
+                    for (int k = 0; k < 4; ++k) {    // (behind the end the limits hide the tokens)
+                        const uint32_t votes = bad ? __ballot_sync(0xffffffffu, slot.block[k * 32 + lane] >= 0) : 0xffffffffu;
+                        if (lane == 0) mt.valid[k] = votes;
+                    }
+                    if (lane == 0) mt.bad = bad;
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&sm.t_full[t % kTileSlots]);
+                }
+                has = more;
+                if (!more) {                         // the end goes on to the loaders
                     __syncwarp();
                     if (lane == 0) mbar_arrive(&sm.t_full[tile % kTileSlots]);
                 }
