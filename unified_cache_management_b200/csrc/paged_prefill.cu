@@ -19,8 +19,8 @@
 //   "dual" item: more than 128 rows, the chains are rows 0-127 and 128-255 and share every token tile;
 //   "single" item: up to 128 rows, the chains take alternate token tiles of the same rows and are merged at the end.
 // Work: items are (request, kv head, row tile), and each is worth its request's number of token tiles.  With at least four
-// items of 256 rows per CTA a CTA takes whole items from its share of the line (row tiles of a request are dealt from both
-// ends, since causal ones get longer); otherwise items have 128 rows and the line is cut evenly, as in paged_attention.cu,
+// items of 256 rows per CTA, none of them large, a CTA takes whole items from its share of the line (row tiles of a request
+// are dealt from both ends, since causal ones get longer); otherwise items have 128 rows and the line is cut evenly, as in paged_attention.cu,
 // with the parts joined by the last CTA to arrive.
 //
 // The running maximum that the rows refer to is only raised when it is exceeded by 2^8, so O rarely has to be scaled
@@ -323,7 +323,11 @@ struct Line {
     int rows;      // rows per item: 256 (whole items) or 128 (cut evenly)
 };
 
-__device__ __forceinline__ int units_of(const AttnRequest& r) { return max(1, (r.len + kTok - 1) / kTok); }
+// An item counts its token tiles, and kItemCost more for reading its queries and writing its rows (about 10 us, where a
+// tile of 128 rows takes 2 to 3).
+constexpr int kItemCost = 4;
+__device__ __forceinline__ int tiles_in(const AttnRequest& r) { return max(1, (r.len + kTok - 1) / kTok); }
+__device__ __forceinline__ int units_of(const AttnRequest& r) { return tiles_in(r) + kItemCost; }
 __device__ __forceinline__ int tiles_of(const AttnParams& p, const AttnRequest& r, int rows)
 {
     return (int)(((int64_t)r.nq * p.G + rows - 1) / rows);
@@ -360,16 +364,17 @@ struct SegmentWalk {
             const int item = (int)(in_b / units);
             const int from = (int)(in_b - (unsigned long long)item * units);
             const unsigned long long item_first = u - from;
-            int to = units;
+            const int in_item = tiles_in(r);
+            int to = in_item;
+            u = item_first + units;
             s.c0 = s.c1 = blockIdx.x;
             if (line.rows == 256) {
-                u = item_first + units;
                 if (from != 0) continue;  // an item belongs to the CTA in whose stretch it begins
             } else {
-                to = (int)min((unsigned long long)units, line.u1 - item_first);
-                u = item_first + to;
+                if (from >= in_item) continue;
+                to = (int)min((unsigned long long)in_item, line.u1 - item_first);
                 s.c0 = (int)(((item_first + 1) * line.n_cta - 1) / line.total);
-                s.c1 = (int)(((item_first + units) * line.n_cta - 1) / line.total);
+                s.c1 = (int)(((item_first + in_item) * line.n_cta - 1) / line.total);
             }
             s.b = b;
             s.q0 = r.q0; s.len = r.len; s.nq = r.nq;
@@ -421,10 +426,13 @@ __global__ void __launch_bounds__(kThreads, 1) tile_kernel(const __grid_constant
     const int per = (p.B + kThreads - 1) / kThreads;
     unsigned long long mine[2] = {0, 0}, before[2];
     unsigned long long whole_items = 0;
+    int largest = 0;
     for (int b = tid * per; b < min(p.B, (tid + 1) * per); ++b) {
         mine[0] += line_of(p, b, 128);
         mine[1] += line_of(p, b, 256);
-        whole_items += (unsigned long long)tiles_of(p, attn_request(p, b), 256) * (unsigned)p.Hkv;
+        const AttnRequest r = attn_request(p, b);
+        whole_items += (unsigned long long)tiles_of(p, r, 256) * (unsigned)p.Hkv;
+        if (r.nq > 0) largest = max(largest, units_of(r));
     }
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
@@ -452,12 +460,14 @@ __global__ void __launch_bounds__(kThreads, 1) tile_kernel(const __grid_constant
     __syncthreads();
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) whole_items += __shfl_xor_sync(0xffffffffu, whole_items, o);
-    if (lane == 0) sm.sums[0][warp] = whole_items;
+    largest = __reduce_max_sync(0xffffffffu, largest);
+    if (lane == 0) { sm.sums[0][warp] = whole_items; sm.sums[1][warp] = largest; }
     __syncthreads();
     whole_items = 0;
-    for (int w = 0; w < kWarps; ++w) whole_items += sm.sums[0][w];
+    for (int w = 0; w < kWarps; ++w) { whole_items += sm.sums[0][w]; largest = max(largest, (int)sm.sums[1][w]); }
     Line line;
-    const int kind = whole_items >= 4ull * gridDim.x ? 1 : 0;
+    // whole items of 256 rows: at least four per CTA, and none that takes more than a third of a CTA's share
+    const int kind = whole_items >= 4ull * gridDim.x && 3ull * largest * gridDim.x <= total[1] ? 1 : 0;
     line.rows = kind ? 256 : 128;
     line.total = total[kind];
     line.n_cta = min((unsigned long long)gridDim.x, line.total);
