@@ -8,16 +8,16 @@
 
 namespace ucmr {
 
-// Workspace: header (device status word first), one arrival counter per CTA, then two partial results per CTA.
-constexpr int kAttnMaxCtas = 512;
-constexpr int kAttnMaxRows = 16;   // query rows of a partial result
-constexpr int kTileMaxCtas = 160;  // the kernel for many rows: one CTA per SM, 128 rows per partial result
-constexpr size_t kAttnCounterBytes = kAttnMaxCtas * sizeof(int32_t);
+// Workspace: header (device status word first), one arrival counter per CTA, then two partial results per CTA: at most
+// kAttnPartRows rows in all, for either kernel.
+constexpr int kAttnMaxSms = 152;
+constexpr int kAttnMaxCtas = 2 * kAttnMaxSms;
+constexpr size_t kAttnPartRows = (size_t)kAttnMaxSms * 2 * 128;
+constexpr size_t kAttnCounterBytes = 512 * sizeof(int32_t);
 
 inline size_t attn_workspace_bytes(int D)
 {
-    constexpr size_t few = (size_t)kAttnMaxCtas * 2 * kAttnMaxRows, many = (size_t)kTileMaxCtas * 2 * 128;
-    return UCMR_WORKSPACE_HEADER_BYTES + kAttnCounterBytes + (few > many ? few : many) * (D + 2) * sizeof(float);
+    return UCMR_WORKSPACE_HEADER_BYTES + kAttnCounterBytes + kAttnPartRows * (D + 2) * sizeof(float);
 }
 
 // Quotients by a fixed divisor (1 .. 2^31 - 1) for numbers below 2^31, without a division: n / d = (hi(m n) + n) >> l with
@@ -110,71 +110,92 @@ template <> struct Out16<__half> {
     }
 };
 
-// Adds up the partial results of one item's CTAs c0 .. c1, in this order, and writes its `rows` rows (from row0 of the
-// request).  CTA c's part lies in slot 2 c, or 2 c + 1 for c0, whose part is the last of its stretch; a slot holds SLOT_ROWS
-// rows of D unnormalised values, then their references, then their sums.  One warp per row: the lanes hold the parts'
-// weights, then D / 32 columns each; eight parts are on their way at a time.
-template <int D, int SLOT_ROWS, int WARPS, typename QT>
-__device__ __forceinline__ void attn_join(const AttnParams& p, int c0, int c1, int q0, int h, int row0, int rows, int warp, int lane)
+// Adds up the partial results of one item's CTAs c0 .. c1, in this order, and writes its rows.  CTA c's part lies in slot 2 c,
+// or 2 c + 1 for c0, whose part is the last of its stretch; a slot holds SLOT_ROWS rows of D unnormalised values, then their
+// references, then their sums.  place(row, token, head): where a row of the slot goes, false if nowhere.  A warp takes four
+// rows at a time: its lanes first hold the parts' weights, then D / 32 columns each; eight values are on their way per lane.
+template <int D, int SLOT_ROWS, int WARPS, typename QT, typename Place>
+__device__ __forceinline__ void attn_join(const AttnParams& p, int c0, int c1, int rows, int warp, int lane, Place place)
 {
-    constexpr int W = D / 32;
+    constexpr int W = D / 32, N = 4;
     const float inf = __uint_as_float(0x7f800000u);
     auto slot = [&](int c) { return p.partial + ((int64_t)c * 2 + (c == c0 ? 1 : 0)) * SLOT_ROWS * (D + 2); };
 #pragma unroll 1
-    for (int r = warp; r < rows; r += WARPS) {
-        float top = -inf;
+    for (int r0 = warp * N; r0 < rows; r0 += WARPS * N) {
+        float top[N], sum[N], v[N][W];
+#pragma unroll
+        for (int n = 0; n < N; ++n) {
+            top[n] = -inf;
+            sum[n] = 0.f;
+#pragma unroll
+            for (int i = 0; i < W; ++i) v[n][i] = 0.f;
+        }
 #pragma unroll 1
-        for (int c = c0 + lane; c <= c1; c += 32) top = fmaxf(top, __ldcg(slot(c) + SLOT_ROWS * D + r));
+        for (int c = c0 + lane; c <= c1; c += 32)
 #pragma unroll
-        for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-        float v[W], sum = 0.f;
+            for (int n = 0; n < N; ++n)
+                if (r0 + n < rows) top[n] = fmaxf(top[n], __ldcg(slot(c) + SLOT_ROWS * D + r0 + n));
 #pragma unroll
-        for (int i = 0; i < W; ++i) v[i] = 0.f;
+        for (int o = 16; o > 0; o >>= 1)
+#pragma unroll
+            for (int n = 0; n < N; ++n) top[n] = fmaxf(top[n], __shfl_xor_sync(0xffffffffu, top[n], o));
 #pragma unroll 1
         for (int first = c0; first <= c1; first += 32) {
             const int c = first + lane;
-            float weight = 0.f;
-            if (c <= c1) {
-                const float m = __ldcg(slot(c) + SLOT_ROWS * D + r), l = __ldcg(slot(c) + SLOT_ROWS * (D + 1) + r);
-                weight = m == -inf ? 0.f : exp2_fast(m - top);
-                sum += m == -inf ? l : weight * l;   // (a sum that is NaN stays one)
+            float weight[N];
+#pragma unroll
+            for (int n = 0; n < N; ++n) {
+                weight[n] = 0.f;
+                if (c <= c1 && r0 + n < rows) {
+                    const float m = __ldcg(slot(c) + SLOT_ROWS * D + r0 + n), l = __ldcg(slot(c) + SLOT_ROWS * (D + 1) + r0 + n);
+                    weight[n] = m == -inf ? 0.f : exp2_fast(m - top[n]);
+                    sum[n] += m == -inf ? l : weight[n] * l;   // (a sum that is NaN stays one)
+                }
             }
             const int here = min(32, c1 - first + 1);
-#pragma unroll 1
-            for (int k = 0; k < here; k += 8) {
-                float x[8][W], f[8];
+#pragma unroll 2
+            for (int k = 0; k < here; ++k) {
+                const float* at = slot(first + k) + r0 * D + lane * W;
+                float x[N][W];
 #pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    f[j] = __shfl_sync(0xffffffffu, weight, (k + j) & 31);
-                    if (k + j >= here) f[j] = 0.f;
-                    const float* at = slot(min(first + k + j, c1)) + r * D + lane * W;
+                for (int n = 0; n < N; ++n) {
+#pragma unroll
+                    for (int i = 0; i < W; ++i) x[n][i] = 0.f;
+                    if (r0 + n >= rows) continue;
                     if constexpr (W == 4) {
-                        const float4 y = __ldcg(reinterpret_cast<const float4*>(at));
-                        x[j][0] = y.x; x[j][1] = y.y; x[j][2] = y.z; x[j][3] = y.w;
+                        const float4 y = __ldcg(reinterpret_cast<const float4*>(at + n * D));
+                        x[n][0] = y.x; x[n][1] = y.y; x[n][2] = y.z; x[n][3] = y.w;
                     } else {
-                        const float2 y = __ldcg(reinterpret_cast<const float2*>(at));
-                        x[j][0] = y.x; x[j][1] = y.y;
+                        const float2 y = __ldcg(reinterpret_cast<const float2*>(at + n * D));
+                        x[n][0] = y.x; x[n][1] = y.y;
                     }
                 }
 #pragma unroll
-                for (int j = 0; j < 8; ++j)
-                    if (f[j] != 0.f)
+                for (int n = 0; n < N; ++n) {
+                    const float f = __shfl_sync(0xffffffffu, weight[n], k);
+                    if (f != 0.f)
 #pragma unroll
-                        for (int i = 0; i < W; ++i) v[i] += f[j] * x[j][i];
+                        for (int i = 0; i < W; ++i) v[n][i] += f * x[n][i];
+                }
             }
         }
 #pragma unroll
-        for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-        const float inv = sum == 0.f ? 0.f : 1.f / sum;
-        const int gr = row0 + r;
-        const int64_t tok = q0 + gr / p.G;
-        const int head = h * p.G + gr % p.G;
-        QT* out = static_cast<QT*>(p.out) + tok * p.os_t + (int64_t)head * p.os_h + lane * W;
-        if constexpr (W == 4)
-            *reinterpret_cast<uint2*>(out) = make_uint2(Out16<QT>::pack(v[0] * inv, v[1] * inv), Out16<QT>::pack(v[2] * inv, v[3] * inv));
-        else
-            *reinterpret_cast<uint32_t*>(out) = Out16<QT>::pack(v[0] * inv, v[1] * inv);
-        if (lane == 0 && p.lse != nullptr) p.lse[tok * p.Hq + head] = sum == 0.f ? -inf : (top + log2f(sum)) * 0.69314718055994531f;
+        for (int o = 16; o > 0; o >>= 1)
+#pragma unroll
+            for (int n = 0; n < N; ++n) sum[n] += __shfl_xor_sync(0xffffffffu, sum[n], o);
+#pragma unroll
+        for (int n = 0; n < N; ++n) {
+            int64_t tok;
+            int head;
+            if (r0 + n >= rows || !place(r0 + n, tok, head)) continue;
+            const float inv = sum[n] == 0.f ? 0.f : 1.f / sum[n];
+            QT* out = static_cast<QT*>(p.out) + tok * p.os_t + (int64_t)head * p.os_h + lane * W;
+            if constexpr (W == 4)
+                *reinterpret_cast<uint2*>(out) = make_uint2(Out16<QT>::pack(v[n][0] * inv, v[n][1] * inv), Out16<QT>::pack(v[n][2] * inv, v[n][3] * inv));
+            else
+                *reinterpret_cast<uint32_t*>(out) = Out16<QT>::pack(v[n][0] * inv, v[n][1] * inv);
+            if (lane == 0 && p.lse != nullptr) p.lse[tok * p.Hq + head] = sum[n] == 0.f ? -inf : (top[n] + log2f(sum[n])) * 0.69314718055994531f;
+        }
     }
 }
 

@@ -848,7 +848,11 @@ __global__ void __launch_bounds__(kThreads, 1) tile_kernel(const __grid_constant
                 bar_sync(1, 256);
                 if (sm.last) {
                     __threadfence();
-                    attn_join<D, 128, 8, QT>(p, c0, c1, s.q0, s.h, s.row0, min(128, s.n_rows - s.row0), warp, lane);
+                    attn_join<D, 128, 8, QT>(p, c0, c1, min(128, s.n_rows - s.row0), warp, lane, [&](int r, int64_t& to, int& of) {
+                        to = s.q0 + (s.row0 + r) / p.G;
+                        of = s.h * p.G + (s.row0 + r) % p.G;
+                        return true;
+                    });
                 }
             }
             bar_sync(1, 256);  // the queries and the merged rows have been used
@@ -1261,7 +1265,7 @@ static int launch(const AttnParams& p, cudaStream_t st)
     cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
     if (e != cudaSuccess) { note_cuda_error(e); (void)cudaGetLastError(); return UCMR_ERR_LAUNCH; }
     const int sms = device_sms();
-    return launch_kernel(kernel, dim3(sms < kTileMaxCtas ? sms : kTileMaxCtas), dim3(kThreads), smem, st, p);
+    return launch_kernel(kernel, dim3(sms < kAttnMaxSms ? sms : kAttnMaxSms), dim3(kThreads), smem, st, p);
 }
 
 }  // namespace tile
