@@ -6,7 +6,6 @@ is no PyTorch or CPU implementation behind these functions.
 """
 from __future__ import annotations
 
-import contextlib
 import ctypes as C
 import math
 from dataclasses import dataclass
@@ -855,13 +854,20 @@ def _same_device(device, **tensors) -> None:
             raise ValueError(f"{name} is on {t.device}, the others are on {device}")
 
 
-def _raw_stream(device) -> int:
-    return torch._C._cuda_getCurrentRawStream(device.index)
+def _call(name: str, index: int, *args) -> None:
+    """Calls the library with device ``index`` current, on that device's current torch stream (the last argument)."""
+    if torch._C._cuda_getDevice() == index:
+        rc = getattr(_l.load_library(), name)(*args, torch._C._cuda_getCurrentRawStream(index))
+    else:
+        with torch.cuda.device(index):
+            rc = getattr(_l.load_library(), name)(*args, torch._C._cuda_getCurrentRawStream(index))
+    if rc:
+        _l.check(rc, name)
 
 
-def _on(device):
-    """Makes the tensors' device the current one for the launch."""
-    return torch.cuda.device(device) if torch.cuda.current_device() != device.index else contextlib.nullcontext()
+# The three operators below are called once or twice per layer and step, so their checks come in two forms: one expression
+# that accepts the usual call in a microsecond or two, and, where it does not hold, the checks one by one, which say what is
+# wrong (or let an unusual but valid call pass).
 
 
 def _angles(positions, inv_freq, tokens: int, dim: int):
@@ -876,27 +882,37 @@ def _angles(positions, inv_freq, tokens: int, dim: int):
     return 2 * inv_freq.numel()
 
 
+def _check_rotary(x, positions, inv_freq, out) -> None:
+    dt = _type_of("x", x, _ACTIVATIONS)
+    _heads("x", x)
+    _angles(positions, inv_freq, x.shape[0], x.shape[2])
+    if out is not None and out is not x:
+        if _type_of("out", out, (x.dtype,)) != dt or out.shape != x.shape:
+            raise ValueError(f"out must be like x: {tuple(x.shape)}, got {tuple(out.shape)}")
+        _heads("out", out)
+    _same_device(x.device, out=out, positions=positions, inv_freq=inv_freq)
+
+
 def rotary(x: torch.Tensor, positions: torch.Tensor, inv_freq: torch.Tensor, *, interleaved: bool = False,
            mscale: float = 1.0, transpose: bool = False, out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """Rotates the first 2 * len(inv_freq) elements of every head of x [T, H, D] (bf16 / fp16) by positions[t] *
     inv_freq; see ``ucmr_rotary``.  ``out`` may be x itself.  ``transpose`` applies the transposed map, which takes the
     gradient of the output to the gradient of x."""
-    dt = _type_of("x", x, _ACTIVATIONS)
-    _heads("x", x)
+    if out is not None or not (isinstance(x, torch.Tensor) and x.is_cuda and x.dtype in _ACTIVATIONS and x.dim() == 3):
+        _check_rotary(x, positions, inv_freq, out)
     t, h, d = x.shape
-    rot = _angles(positions, inv_freq, t, d)
+    xs, index, rot, kind = x.stride(), x.get_device(), 2 * inv_freq.shape[0] if inv_freq is not None else 0, None
+    if positions is not None:
+        kind = positions.dtype
+    if not (xs[2] == 1 and 0 < rot <= d and inv_freq.dim() == 1 and inv_freq.dtype == torch.float64 and inv_freq.stride(0) == 1 and
+            (kind == torch.int64 or kind == torch.int32) and positions.shape == (t,) and positions.is_contiguous() and
+            inv_freq.get_device() == index == positions.get_device()):
+        _check_rotary(x, positions, inv_freq, out)
     if out is None:
         out = torch.empty((t, h, d), dtype=x.dtype, device=x.device)
-    elif out is not x:
-        if _type_of("out", out, (x.dtype,)) != dt or out.shape != x.shape:
-            raise ValueError(f"out must be like x: {tuple(x.shape)}, got {tuple(out.shape)}")
-        _heads("out", out)
-    _same_device(x.device, out=out, positions=positions, inv_freq=inv_freq)
-    with _on(x.device):
-        _l.check(_l.load_library().ucmr_rotary(
-            x.data_ptr(), out.data_ptr(), t, h, d, x.stride(0), x.stride(1), out.stride(0), out.stride(1), dt,
-            positions.data_ptr(), positions.dtype == torch.int64, inv_freq.data_ptr(), rot, bool(interleaved),
-            float(mscale), bool(transpose), _raw_stream(x.device)), "ucmr_rotary")
+    os = out.stride()
+    _call("ucmr_rotary", index, x.data_ptr(), out.data_ptr(), t, h, d, xs[0], xs[1], os[0], os[1], _TYPES[x.dtype],
+          positions.data_ptr(), kind == torch.int64, inv_freq.data_ptr(), rot, bool(interleaved), float(mscale), bool(transpose))
     return out
 
 
@@ -930,30 +946,94 @@ def kv_append(k: torch.Tensor, v: torch.Tensor, slot_mapping: torch.Tensor, k_ca
     is returned; made if None), and the rotated keys also go to ``k_out`` in 16 bits (for the hash encode).  Caches of
     k's dtype hold the rows; caches of float8_e4m3fn hold codes, with ``k_scale`` / ``v_scale`` float32 [NB, Hkv].  See
     ``ucmr_kv_append`` for how a block's scale starts and grows."""
+    if not _plain_append(k, v, slot_mapping, k_cache, v_cache, k_scale, v_scale, positions, inv_freq, q, q_out, k_out):
+        _check_append(k, v, slot_mapping, k_cache, v_cache, k_scale, v_scale, positions, inv_freq, q, q_out, k_out)
+    t, hkv, d = k.shape
+    ks, vs, kc, vc = k.stride(), v.stride(), k_cache.stride(), v_cache.stride()
+    qp = qop = kop = pp = fp = None
+    qs = qos = kos = (0, 0)
+    hq = rot = p64 = 0
+    if positions is not None:
+        pp, p64, fp, rot = positions.data_ptr(), positions.dtype == torch.int64, inv_freq.data_ptr(), 2 * inv_freq.shape[0]
+    if q is not None:
+        if q_out is None:
+            q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        qp, qop, qs, qos, hq = q.data_ptr(), q_out.data_ptr(), q.stride(), q_out.stride(), q.shape[1]
+    if k_out is not None:
+        kop, kos = k_out.data_ptr(), k_out.stride()
+    _call("ucmr_kv_append", k.get_device(), k.data_ptr(), ks[0], ks[1], v.data_ptr(), vs[0], vs[1], t, hkv, d, _TYPES[k.dtype],
+          slot_mapping.data_ptr(), slot_mapping.dtype == torch.int64, k_cache.data_ptr(), kc[0], kc[1], kc[2],
+          v_cache.data_ptr(), vc[0], vc[1], vc[2], k_cache.shape[0], k_cache.shape[1], _TYPES[k_cache.dtype],
+          None if k_scale is None else k_scale.data_ptr(), None if v_scale is None else v_scale.data_ptr(), pp, p64, fp, rot,
+          bool(interleaved), float(mscale), qp, hq, qs[0], qs[1], qop, qos[0], qos[1], kop, kos[0], kos[1])
+    return q_out
+
+
+def _rows(t, device: int, dtype, tokens: int, dim: int) -> bool:
+    """t is [tokens, *, dim] of the dtype on the device, its rows contiguous."""
+    return t.dtype == dtype and t.dim() == 3 and t.shape[0] == tokens and t.shape[2] == dim and t.stride(2) == 1 and \
+        t.get_device() == device
+
+
+def _caches(k_cache, v_cache, k_scale, v_scale, device: int, dtype, hkv: int, dim: int) -> bool:
+    shape, kind = k_cache.shape, k_cache.dtype
+    if not (len(shape) == 4 and shape[2] == hkv and shape[3] == dim and v_cache.shape == shape and v_cache.dtype == kind and
+            k_cache.stride(3) == 1 == v_cache.stride(3) and k_cache.get_device() == device == v_cache.get_device()):
+        return False
+    if kind == dtype:
+        return k_scale is None and v_scale is None
+    if kind != torch.float8_e4m3fn or k_scale is None or v_scale is None:
+        return False
+    scales = (shape[0], hkv)
+    return k_scale.shape == scales and v_scale.shape == scales and k_scale.dtype == torch.float32 == v_scale.dtype and \
+        k_scale.is_contiguous() and v_scale.is_contiguous() and k_scale.get_device() == device == v_scale.get_device()
+
+
+def _plain_append(k, v, slot_mapping, k_cache, v_cache, k_scale, v_scale, positions, inv_freq, q, q_out, k_out) -> bool:
+    """The usual call: everything on one device, shapes and types as documented."""
+    for x in (k, v, slot_mapping, k_cache, v_cache):
+        if not isinstance(x, torch.Tensor):
+            return False
+    if not (k.is_cuda and k.dtype in _ACTIVATIONS and k.dim() == 3):
+        return False
+    device, dtype, (t, hkv, d) = k.get_device(), k.dtype, k.shape
+    if not (k.stride(2) == 1 and v.shape == k.shape and v.dtype == dtype and v.stride(2) == 1 and v.get_device() == device and
+            slot_mapping.dtype in _INDEXES and slot_mapping.shape == (t,) and slot_mapping.is_contiguous() and
+            slot_mapping.get_device() == device and _caches(k_cache, v_cache, k_scale, v_scale, device, dtype, hkv, d)):
+        return False
+    if inv_freq is None or positions is None:
+        return inv_freq is None and positions is None and q is None and q_out is None and k_out is None
+    if not (inv_freq.dim() == 1 and inv_freq.dtype == torch.float64 and 0 < 2 * inv_freq.shape[0] <= d and inv_freq.stride(0) == 1 and
+            positions.dtype in _INDEXES and positions.shape == (t,) and positions.is_contiguous() and
+            inv_freq.get_device() == device == positions.get_device()):
+        return False
+    if q is not None and not _rows(q, device, dtype, t, d):
+        return False
+    if q_out is not None and (q is None or q_out.shape != q.shape or not _rows(q_out, device, dtype, t, d)):
+        return False
+    return k_out is None or (k_out.shape == k.shape and _rows(k_out, device, dtype, t, d) and (k_out.data_ptr() != k.data_ptr() or t == 0))
+
+
+def _check_append(k, v, slot_mapping, k_cache, v_cache, k_scale, v_scale, positions, inv_freq, q, q_out, k_out) -> None:
     dt = _type_of("k", k, _ACTIVATIONS)
     if _type_of("v", v, (k.dtype,)) != dt or v.shape != k.shape:
         raise ValueError("k and v must agree in shape and dtype")
     _heads("k", k)
     _heads("v", v)
     t, hkv, d = k.shape
-    kind = _check_cache(k_cache, v_cache, k_scale, v_scale, k.dtype, hkv, d)
+    _check_cache(k_cache, v_cache, k_scale, v_scale, k.dtype, hkv, d)
     _need_cuda("slot_mapping", slot_mapping, _INDEXES)
     if slot_mapping.shape != (t,):
         raise ValueError(f"slot_mapping must be [{t}], got {tuple(slot_mapping.shape)}")
-    rot = 0
     if inv_freq is not None or positions is not None:
-        rot = _angles(positions, inv_freq, t, d)
+        _angles(positions, inv_freq, t, d)
     elif q is not None or k_out is not None:
         raise ValueError("q and k_out need positions and inv_freq")
-    hq = 0
     if q is not None:
         _type_of("q", q, (k.dtype,))
         _heads("q", q)
         if q.shape[0] != t or q.shape[2] != d:
             raise ValueError(f"q must be [{t}, Hq, {d}], got {tuple(q.shape)}")
-        hq = q.shape[1]
-        if q_out is None:
-            q_out = torch.empty((t, hq, d), dtype=q.dtype, device=q.device)
     elif q_out is not None:
         raise ValueError("q_out without q")
     for name, o, like in (("q_out", q_out, q), ("k_out", k_out, k)):
@@ -964,24 +1044,8 @@ def kv_append(k: torch.Tensor, v: torch.Tensor, slot_mapping: torch.Tensor, k_ca
                 raise ValueError(f"{name} must be {tuple(like.shape)}, got {tuple(o.shape)}")
     if k_out is not None and k_out.data_ptr() == k.data_ptr() and t > 0:
         raise ValueError("k_out must not be k: the keys are still read while it is written")
-    dev = k.device
-    _same_device(dev, v=v, slot_mapping=slot_mapping, k_cache=k_cache, v_cache=v_cache, k_scale=k_scale, v_scale=v_scale,
+    _same_device(k.device, v=v, slot_mapping=slot_mapping, k_cache=k_cache, v_cache=v_cache, k_scale=k_scale, v_scale=v_scale,
                  positions=positions, inv_freq=inv_freq, q=q, q_out=q_out, k_out=k_out)
-
-    def ptr(x):
-        return None if x is None else x.data_ptr()
-
-    def strides(x):
-        return (0, 0) if x is None else (x.stride(0), x.stride(1))
-    with _on(dev):
-        _l.check(_l.load_library().ucmr_kv_append(
-            k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0), v.stride(1), t, hkv, d, dt,
-            slot_mapping.data_ptr(), slot_mapping.dtype == torch.int64, k_cache.data_ptr(), *k_cache.stride()[:3],
-            v_cache.data_ptr(), *v_cache.stride()[:3], k_cache.shape[0], k_cache.shape[1], kind, ptr(k_scale), ptr(v_scale),
-            ptr(positions), positions is not None and positions.dtype == torch.int64, ptr(inv_freq), rot,
-            bool(interleaved), float(mscale), ptr(q), hq, *strides(q), ptr(q_out), *strides(q_out), ptr(k_out),
-            *strides(k_out), _raw_stream(dev)), "ucmr_kv_append")
-    return q_out
 
 
 def paged_attention_workspace_bytes(head_dim: int) -> int:
@@ -1006,62 +1070,95 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     chosen).  One query token per request (T = B), or request b's tokens at query_start[b] .. query_start[b+1] with
     ``max_query_len`` at least the largest count.  ``scale`` defaults to 1 / sqrt(D).  Returns out, or (out, lse) when the
     log-sum-exp (float32 [T, Hq]) is wanted.  Rows outside every request are left as they were."""
+    if not _plain_attention(q, k_cache, v_cache, block_table, seq_lens, k_scale, v_scale, query_start, max_query_len, out, lse, workspace):
+        _check_attention(q, k_cache, v_cache, block_table, seq_lens, k_scale, v_scale, query_start, max_query_len, out, lse, workspace)
+    t, hq, d = q.shape
+    nb, bs, hkv, _ = k_cache.shape
+    table = block_table.stride()
+    bt_h = table[1] if len(table) == 3 and block_table.shape[1] > 1 else 0
+    if out is None:
+        out = torch.empty((t, hq, d), dtype=q.dtype, device=q.device)
+    if lse is None and want_lse:
+        lse = torch.empty((t, hq), dtype=torch.float32, device=q.device)
+    if workspace is None:
+        workspace = new_attention_workspace(d, q.device)
+    qs, os, kc, vc = q.stride(), out.stride(), k_cache.stride(), v_cache.stride()
+    _call("ucmr_paged_attention", q.get_device(), q.data_ptr(), t, hq, d, qs[0], qs[1], _TYPES[q.dtype], k_cache.data_ptr(), kc[0], kc[1],
+          kc[2], v_cache.data_ptr(), vc[0], vc[1], vc[2], nb, bs, hkv, _TYPES[k_cache.dtype],
+          None if k_scale is None else k_scale.data_ptr(), None if v_scale is None else v_scale.data_ptr(),
+          block_table.data_ptr(), block_table.shape[-1], table[0], bt_h, seq_lens.data_ptr(),
+          None if query_start is None else query_start.data_ptr(), 1 if query_start is None else int(max_query_len),
+          block_table.shape[0], d ** -0.5 if scale is None else float(scale), bool(causal), out.data_ptr(), os[0], os[1],
+          None if lse is None else lse.data_ptr(), workspace.data_ptr(), workspace.numel() * workspace.element_size())
+    return out if lse is None else (out, lse)
+
+
+def _plain_attention(q, k_cache, v_cache, block_table, seq_lens, k_scale, v_scale, query_start, max_query_len, out, lse, workspace) -> bool:
+    """The usual call: everything on one device, shapes and types as documented."""
+    for x in (q, k_cache, v_cache, block_table, seq_lens):
+        if not isinstance(x, torch.Tensor):
+            return False
+    if not (q.is_cuda and q.dtype in _ACTIVATIONS and q.dim() == 3 and k_cache.dim() == 4):
+        return False
+    device, dtype, (t, hq, d), hkv = q.get_device(), q.dtype, q.shape, k_cache.shape[2]
+    shape = block_table.shape
+    b = shape[0]
+    if not (q.stride(2) == 1 and hkv > 0 and hq > 0 and hq % hkv == 0 and
+            _caches(k_cache, v_cache, k_scale, v_scale, device, dtype, hkv, d) and
+            block_table.dtype == torch.int32 and (len(shape) == 2 or (len(shape) == 3 and (shape[1] == hkv or shape[1] == 1))) and
+            block_table.stride(-1) == 1 and seq_lens.dtype == torch.int32 and seq_lens.shape == (b,) and seq_lens.is_contiguous() and
+            block_table.get_device() == device == seq_lens.get_device()):
+        return False
+    if query_start is None:
+        if t != b:
+            return False
+    elif not (query_start.dtype == torch.int32 and query_start.shape == (b + 1,) and query_start.is_contiguous() and
+              query_start.get_device() == device and max_query_len is not None and max_query_len >= 0):
+        return False
+    if out is not None and not (out.shape == q.shape and _rows(out, device, dtype, t, d)):
+        return False
+    if lse is not None and not (lse.shape == (t, hq) and lse.dtype == torch.float32 and lse.is_contiguous() and lse.get_device() == device):
+        return False
+    return workspace is None or (workspace.is_contiguous() and workspace.get_device() == device)
+
+
+def _check_attention(q, k_cache, v_cache, block_table, seq_lens, k_scale, v_scale, query_start, max_query_len, out, lse, workspace) -> None:
     dt = _type_of("q", q, _ACTIVATIONS)
     _heads("q", q)
     t, hq, d = q.shape
     if not isinstance(k_cache, torch.Tensor) or k_cache.dim() != 4:
         raise ValueError("k_cache must be [NB, BS, Hkv, D]")
-    nb, bs, hkv, _ = k_cache.shape
-    kind = _check_cache(k_cache, v_cache, k_scale, v_scale, q.dtype, hkv, d)
+    hkv = k_cache.shape[2]
+    _check_cache(k_cache, v_cache, k_scale, v_scale, q.dtype, hkv, d)
     if hkv == 0 or hq == 0 or hq % hkv:
         raise ValueError("number of query heads must be a multiple of the kv heads")
     _need_cuda("block_table", block_table, torch.int32, contiguous=False)
     if block_table.dim() not in (2, 3) or (block_table.stride(-1) != 1 and block_table.shape[-1] > 1):
         raise ValueError("block_table must be [B, max_blocks] or [B, Hkv, max_blocks] with a unit inner stride")
-    b, mb = block_table.shape[0], block_table.shape[-1]
+    b = block_table.shape[0]
     if block_table.dim() == 3 and block_table.shape[1] not in (1, hkv):
         raise ValueError(f"a per-head block_table must be [B, {hkv}, max_blocks], got {tuple(block_table.shape)}")
-    bt_h = block_table.stride(1) if block_table.dim() == 3 and block_table.shape[1] > 1 else 0
     _need_cuda("seq_lens", seq_lens, torch.int32)
     if seq_lens.shape != (b,):
         raise ValueError(f"seq_lens must be [{b}], got {tuple(seq_lens.shape)}")
     if query_start is None:
         if t != b:
             raise ValueError(f"{t} query tokens for {b} requests: give query_start and max_query_len")
-        max_query_len = 1
     else:
         _need_cuda("query_start", query_start, torch.int32)
         if query_start.shape != (b + 1,):
             raise ValueError(f"query_start must be [{b + 1}], got {tuple(query_start.shape)}")
         if max_query_len is None or max_query_len < 0:
             raise ValueError("query_start needs max_query_len, the largest number of query tokens of a request")
-    if out is None:
-        out = torch.empty((t, hq, d), dtype=q.dtype, device=q.device)
-    else:
+    if out is not None:
         if _type_of("out", out, (q.dtype,)) != dt or out.shape != q.shape:
             raise ValueError(f"out must be like q: {tuple(q.shape)}, got {tuple(out.shape)}")
         _heads("out", out)
     if lse is not None:
-        want_lse = True
         _need_cuda("lse", lse, torch.float32)
         if lse.shape != (t, hq):
             raise ValueError(f"lse must be [{t}, {hq}], got {tuple(lse.shape)}")
-    elif want_lse:
-        lse = torch.empty((t, hq), dtype=torch.float32, device=q.device)
-    dev = q.device
-    if workspace is None:
-        workspace = new_attention_workspace(d, dev)
-    else:
+    if workspace is not None:
         _need_cuda("workspace", workspace)
-    _same_device(dev, k_cache=k_cache, v_cache=v_cache, k_scale=k_scale, v_scale=v_scale, block_table=block_table,
+    _same_device(q.device, k_cache=k_cache, v_cache=v_cache, k_scale=k_scale, v_scale=v_scale, block_table=block_table,
                  seq_lens=seq_lens, query_start=query_start, out=out, lse=lse, workspace=workspace)
-    with _on(dev):
-        _l.check(_l.load_library().ucmr_paged_attention(
-            q.data_ptr(), t, hq, d, q.stride(0), q.stride(1), dt, k_cache.data_ptr(), *k_cache.stride()[:3],
-            v_cache.data_ptr(), *v_cache.stride()[:3], nb, bs, hkv, kind, None if k_scale is None else k_scale.data_ptr(),
-            None if v_scale is None else v_scale.data_ptr(), block_table.data_ptr(), mb, block_table.stride(0), bt_h,
-            seq_lens.data_ptr(), None if query_start is None else query_start.data_ptr(), int(max_query_len), b,
-            float(d ** -0.5 if scale is None else scale), bool(causal), out.data_ptr(), out.stride(0), out.stride(1),
-            None if lse is None else lse.data_ptr(), workspace.data_ptr(), workspace.numel() * workspace.element_size(),
-            _raw_stream(dev)), "ucmr_paged_attention")
-    return (out, lse) if want_lse else out
