@@ -150,6 +150,21 @@ inline int launch_kernel_cluster(void (*kernel)(KArgs...), dim3 grid, dim3 block
     return UCMR_OK;
 }
 
+// Quotients by a fixed divisor (1 .. 2^31 - 1) for numbers below 2^31, without a division: n / d = (hi(m n) + n) >> l with
+// l = ceil(log2 d), m = floor(2^32 (2^l - d) / d) + 1.
+struct FastDiv {
+    uint32_t m, l;
+    static FastDiv by(uint32_t d)
+    {
+        uint32_t l = 0;
+        while (l < 31 && (1u << l) < d) ++l;
+        return FastDiv{(uint32_t)((((1ull << l) - d) << 32) / d + 1), l};
+    }
+#ifdef __CUDACC__
+    __device__ __forceinline__ int div(int n) const { return (int)((__umulhi(m, (uint32_t)n) + (uint32_t)n) >> l); }
+#endif
+};
+
 // Time bound of every spin-wait in this library.  A wait that runs out sets UCMR_DEV_WAIT_TIMEOUT in
 // the status word and the kernel winds down without touching the data.
 constexpr unsigned long long kWaitLimitNs = 1000ull * 1000ull * 1000ull;  // 1 s

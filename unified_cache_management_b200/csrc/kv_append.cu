@@ -22,7 +22,7 @@
 // The walk costs T / chunk * head groups * T slot reads out of L2: 134 MB for 32768 tokens in chunks of 128 with two head
 // groups, next to 740 MB of HBM traffic that the call cannot do without.
 //
-// Keys and values of a candidate go to the two halves of the CTA.  Each half (128 threads) takes the block's rows of one
+// Keys and values of a candidate go to the two halves of the CTA.  Each half (256 threads) takes the block's rows of one
 // head as a tile of up to 16384 elements held in registers as 16-bit values: load, rotate, largest value, scale, rotate
 // again and store.  Blocks with more elements per head take several tiles; they are walked forwards for the largest value
 // and backwards for the codes, so that the last tile is not read twice.  HBM-bound: 2 bytes read and 1 written per element.
@@ -34,9 +34,8 @@ namespace ucmr {
 
 int device_sms();
 
-constexpr int kAppHalf = 128;              // threads per half
-constexpr int kAppTile = 16384;            // elements per tile: eight items of 16 per thread
-constexpr int kAppItems = kAppTile / 16 / kAppHalf;
+constexpr int kAppHalf = 256;              // threads per half
+constexpr int kAppTile = 16384;            // elements of a head whose cosines and sines are in shared memory: 64 KB
 constexpr int kAppMaxChunk = 128;
 constexpr int kAppMaxBlock = 1024;         // rows per block
 constexpr int kAppList = 1024;             // (candidate, token) pairs that the walk may find before it is repeated per candidate
@@ -52,6 +51,7 @@ struct AppendJob {
     int64_t T, NB;
     int BS, Hkv, D;
     int chunk, heads_per_cta, head_tiles;
+    FastDiv by_row, by_block;   // divisions by the items of a row, D / 16, and by BS
 };
 
 struct AppendParams {
@@ -94,12 +94,6 @@ __device__ __forceinline__ void item_values(uint4 va, uint4 vb, bool turn, const
     }
 }
 
-__device__ __forceinline__ float finite_abs(float v)
-{
-    const float m = fabsf(v);
-    return m <= 3.402823466e38f ? m : 0.f;  // (false for NaN)
-}
-
 // Exponent e of the scale 2^e for a largest value `m` > 0: 448 = 1.75 * 2^8.  Kept at -126 or more, so that the scale and
 // its reciprocal are normal numbers.
 __device__ __forceinline__ float scale_for(float m)
@@ -111,16 +105,21 @@ __device__ __forceinline__ float scale_for(float m)
     return __uint_as_float((uint32_t)(e + 127) << 23);
 }
 
-// Reciprocal of a scale: exact for a power of two.  A scale that a caller brought may be anything else.
-__device__ __forceinline__ float inverse_scale(float s) { return s > 0.f ? 1.0f / s : 0.f; }
+// Reciprocal of a scale: exact for a power of two.  A scale that a caller brought may be anything else; kept finite, so that
+// zeros stay zeros.
+__device__ __forceinline__ float inverse_scale(float s) { return s > 0.f ? fminf(1.0f / s, 3.402823466e38f) : 0.f; }
 
+// Four codes, rounded to nearest, |values| up to 448 or NaN.  ODD: values may be infinite, which the saturating conversion
+// would make 448: they become NaN.
+template <bool ODD>
 __device__ __forceinline__ uint32_t to_e4m3x4(float a, float b, float c, float d)
 {
-    // saturating conversion, two values at a time (the second operand goes to the low byte); infinities become NaN
-    const float inf = __uint_as_float(0x7f800000u), nan = __uint_as_float(0x7fffffffu);
-    a = fabsf(a) == inf ? nan : a; b = fabsf(b) == inf ? nan : b;
-    c = fabsf(c) == inf ? nan : c; d = fabsf(d) == inf ? nan : d;
-    uint16_t lo, hi;
+    if (ODD) {
+        const float inf = __uint_as_float(0x7f800000u), nan = __uint_as_float(0x7fffffffu);
+        a = fabsf(a) == inf ? nan : a; b = fabsf(b) == inf ? nan : b;
+        c = fabsf(c) == inf ? nan : c; d = fabsf(d) == inf ? nan : d;
+    }
+    uint16_t lo, hi;  // (the second operand goes to the low byte)
     asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(lo) : "f"(b), "f"(a));
     asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(hi) : "f"(d), "f"(c));
     return (uint32_t)lo | ((uint32_t)hi << 16);
@@ -135,13 +134,11 @@ __device__ __forceinline__ void from_e4m3x4(uint32_t w, float (&f)[4])
     f[0] = a.x; f[1] = a.y; f[2] = b.x; f[3] = b.y;
 }
 
-// Codes of eight values; an infinite value times a scale of 0 or less stays non-finite on the way.
+template <bool ODD>
 __device__ __forceinline__ uint2 codes8(const float (&v)[8], float inv)
 {
-    float s[8];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) s[i] = v[i] == 0.f ? v[i] : v[i] * inv;
-    return make_uint2(to_e4m3x4(s[0], s[1], s[2], s[3]), to_e4m3x4(s[4], s[5], s[6], s[7]));
+    return make_uint2(to_e4m3x4<ODD>(v[0] * inv, v[1] * inv, v[2] * inv, v[3] * inv),
+                      to_e4m3x4<ODD>(v[4] * inv, v[5] * inv, v[6] * inv, v[7] * inv));
 }
 
 // Shared memory of the store: cosines and sines of a tile's rows (rows * rot/16 * 64 bytes), then the control words.
@@ -155,137 +152,148 @@ struct AppendCtl {
     int n_cand, n_list, n_rows;
     int row_token[kAppMaxBlock];   // token of each row of the block in hand, -1 = not written
     int rows[kAppMaxBlock];        // the rows that are written
-    uint32_t big[2][2];            // largest value of a half's rows, as bits; heads take the two words in turn
-    int warp_count[8];
+    int tokens[kAppMaxBlock];      // and their tokens
+    uint32_t big[2][4];            // largest value of a half's rows, as bits, and largest finite one; heads take them in turn
+    int warp_count[kAppMaxChunk / 32];
 };
 
 __device__ __forceinline__ uint32_t filter_bit(int64_t block) { return ((uint32_t)block * 2654435761u) >> 22; }
 
-// One half of the CTA stores its kind (0 keys, 1 values) of one block for the CTA's heads.
-template <typename T, bool CODES>
-__device__ void store_block(const AppendParams& p, int kind, int64_t block, int n_rows, bool anew, int h0, int nh,
+// Cosines and sines of the rows [r0, r0 + nr) of the block in hand, by `threads` threads.
+__device__ __forceinline__ void fill_tile(const AppendParams& p, float4* cs, const AppendCtl* ctl, int r0, int nr, int tid, int threads)
+{
+    const int np = p.ang.rot / 2, chunks = p.ang.rot / 16;
+    for (int i = tid; i < nr * np; i += threads) {
+        const int row = i / np;
+        fill_cos_sin(cs, p.ang, load_index(p.ang.positions, p.ang.pos_is_int64, ctl->tokens[r0 + row]), row, i - row * np, chunks);
+    }
+}
+
+// One half of the CTA stores its kind (0 keys, 1 values) of one block for the CTA's heads.  The cosines of a block that is one
+// tile are there already.
+template <typename T, bool CODES, bool TURN>
+__device__ __forceinline__ void store_block(const AppendParams& p, int kind, int64_t block, int n_rows, bool anew, int h0, int nh,
                             float4* cs, AppendCtl* ctl)
 {
     const AppendJob& j = p.store;
     const int tid = threadIdx.x & (kAppHalf - 1);
     const int per_row = j.D / 16;
-    const bool rotated = kind == 0 && p.ang.inv_freq != nullptr;
-    const int turn_chunks = rotated ? p.ang.rot / 16 : 0, np = p.ang.rot / 2;
+    const int turn_chunks = TURN ? p.ang.rot / 16 : 0;
     const int tile_rows = kAppTile / j.D;
     const int tiles = (n_rows + tile_rows - 1) / tile_rows;
     const T* x = static_cast<const T*>(j.x[kind]);
-    int table_of = -1;  // tile whose cosines are in shared memory
+    int table_of = tiles == 1 ? 0 : -1;  // tile whose cosines are in shared memory
+    const uint32_t inf_bits = 0x7f800000u;
 
     for (int hi = 0; hi < nh; ++hi) {
         const int h = h0 + hi;
-        uint4 va[kAppItems], vb[kAppItems];
         float big = 0.f;
         float inv = 0.f;
-        // pass 0: tiles 0 .. n-1, largest value; pass 1: tiles n-1 .. 0, store (the last tile is still in registers).
-        // 16-bit caches need pass 1 alone.
-        for (int pass = CODES ? 0 : 1; pass < 2; ++pass) {
-            for (int k = 0; k < tiles; ++k) {
-                const int tile = pass == 0 ? k : tiles - 1 - k;
-                const int r0 = tile * tile_rows, nr = min(tile_rows, n_rows - r0);
-                const int items = nr * per_row;
-                if (!(CODES && pass == 1 && k == 0)) {
-#pragma unroll
-                    for (int u = 0; u < kAppItems; ++u) {
-                        const int i = u * kAppHalf + tid;
-                        if (i < items) {
-                            const int r = i / per_row;
-                            const ItemPlace at = item_place(rotated, p.ang, i - r * per_row);
-                            const T* src = x + (int64_t)ctl->row_token[ctl->rows[r0 + r]] * j.xs_t[kind] + (int64_t)h * j.xs_h[kind];
-                            va[u] = *reinterpret_cast<const uint4*>(src + at.first);
-                            vb[u] = *reinterpret_cast<const uint4*>(src + at.second);
-                        }
-                    }
-                }
-                if (rotated && table_of != tile) {
+        // f(values, raw values, row, item) for each of the block's items; once for the largest value and once more, out of L2,
+        // for the codes: holding them in registers in between left too few warps to hide the latencies (238 -> see below).
+        auto walk = [&](auto&& f) {
+            for (int tile = 0; tile < tiles; ++tile) {
+                const int r0 = tile * tile_rows, items = min(tile_rows, n_rows - r0) * per_row;
+                if (TURN && table_of != tile) {
                     half_sync(kind);  // nobody reads the old cosines any more
-                    for (int i = tid; i < nr * np; i += kAppHalf) {
-                        const int row = i / np;
-                        fill_cos_sin(cs, p.ang, load_index(p.ang.positions, p.ang.pos_is_int64, ctl->row_token[ctl->rows[r0 + row]]),
-                                     row, i - row * np, turn_chunks);
-                    }
+                    fill_tile(p, cs, ctl, r0, min(tile_rows, n_rows - r0), tid, kAppHalf);
                     half_sync(kind);
                     table_of = tile;
                 }
-#pragma unroll
-                for (int u = 0; u < kAppItems; ++u) {
-                    const int i = u * kAppHalf + tid;
-                    if (i < items) {
-                        const int r = i / per_row, ch = i - r * per_row;
-                        float a[8], b[8];
-                        item_values<T>(va[u], vb[u], ch < turn_chunks, cs + r * 4 * turn_chunks + ch, turn_chunks,
-                                       p.ang.interleaved, a, b);
-                        if (pass == 0) {
-#pragma unroll
-                            for (int e = 0; e < 8; ++e) big = fmaxf(big, fmaxf(finite_abs(a[e]), finite_abs(b[e])));
-                        } else {
-                            const ItemPlace at = item_place(rotated, p.ang, ch);
-                            const int64_t dst = block * j.cs_b[kind] + (int64_t)ctl->rows[r0 + r] * j.cs_t[kind] + (int64_t)h * j.cs_h[kind];
-                            if constexpr (CODES) {
-                                uint8_t* o = static_cast<uint8_t*>(j.cache[kind]) + dst;
-                                const uint2 c0 = codes8(a, inv), c1 = codes8(b, inv);
-                                if (at.second == at.first + 8) {
-                                    *reinterpret_cast<uint4*>(o + at.first) = make_uint4(c0.x, c0.y, c1.x, c1.y);
-                                } else {
-                                    *reinterpret_cast<uint2*>(o + at.first) = c0;
-                                    *reinterpret_cast<uint2*>(o + at.second) = c1;
-                                }
-                            } else {
-                                T* o = static_cast<T*>(j.cache[kind]) + dst;
-                                uint4 w;
-                                w.x = Half2<T>::from_float(a[0], a[1]); w.y = Half2<T>::from_float(a[2], a[3]);
-                                w.z = Half2<T>::from_float(a[4], a[5]); w.w = Half2<T>::from_float(a[6], a[7]);
-                                *reinterpret_cast<uint4*>(o + at.first) = ch < turn_chunks ? w : va[u];
-                                w.x = Half2<T>::from_float(b[0], b[1]); w.y = Half2<T>::from_float(b[2], b[3]);
-                                w.z = Half2<T>::from_float(b[4], b[5]); w.w = Half2<T>::from_float(b[6], b[7]);
-                                *reinterpret_cast<uint4*>(o + at.second) = ch < turn_chunks ? w : vb[u];
-                            }
-                        }
-                    }
+#pragma unroll 2
+                for (int i = tid; i < items; i += kAppHalf) {
+                    const int r = j.by_row.div(i), ch = i - r * per_row;
+                    const ItemPlace at = item_place(TURN, p.ang, ch);
+                    const T* src = x + (int64_t)ctl->tokens[r0 + r] * j.xs_t[kind] + (int64_t)h * j.xs_h[kind];
+                    const uint4 va = *reinterpret_cast<const uint4*>(src + at.first), vb = *reinterpret_cast<const uint4*>(src + at.second);
+                    float a[8], b[8];
+                    item_values<T>(va, vb, TURN && ch < turn_chunks, cs + r * 4 * turn_chunks + ch, turn_chunks, p.ang.interleaved, a, b);
+                    f(a, b, va, vb, ctl->rows[r0 + r], ch);
                 }
             }
-            if constexpr (CODES) {
-                if (pass == 1) break;
-                // the half's largest value -> scale (every thread computes the same), old codes re-rounded if it grows
-                const uint32_t m = __reduce_max_sync(0xffffffffu, __float_as_uint(big));
-                float* scale = j.scale[kind] + block * j.Hkv + h;
-                const float old = anew ? 0.f : *scale;
-                // (the word was last read two heads ago, on the other side of the previous head's barriers)
-                uint32_t* word = &ctl->big[kind][hi & 1];
-                if (tid == 0) *word = 0;
-                half_sync(kind);  // (also: everybody has read the old scale)
-                if ((tid & 31) == 0) atomicMax(word, m);
+        };
+        if constexpr (CODES) {
+            walk([&](const float (&a)[8], const float (&b)[8], const uint4&, const uint4&, int, int) {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) big = fmaxf(big, fmaxf(fabsf(a[e]), fabsf(b[e])));   // (NaN has no say)
+            });
+            // The half's largest value -> scale (every thread computes the same); old codes are re-rounded if it grows.  The
+            // words were last read two heads ago, on the other side of the previous head's barriers.
+            uint32_t* word = &ctl->big[kind][hi & 1];
+            float* scale = j.scale[kind] + block * j.Hkv + h;
+            const float old = anew ? 0.f : *scale;
+            if (tid == 0) { word[0] = 0; word[2] = 0; }
+            half_sync(kind);  // (also: everybody has read the old scale)
+            const uint32_t m = __reduce_max_sync(0xffffffffu, __float_as_uint(big));
+            if ((tid & 31) == 0) atomicMax(word, m);
+            half_sync(kind);
+            uint32_t largest = word[0];
+            const bool odd = largest >= inf_bits;
+            if (odd) {        // an infinity among them: once more without
+                float fin = 0.f;
+                walk([&](const float (&a)[8], const float (&b)[8], const uint4&, const uint4&, int, int) {
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        const float ea = fabsf(a[e]), eb = fabsf(b[e]);
+                        if (ea <= 3.402823466e38f) fin = fmaxf(fin, ea);
+                        if (eb <= 3.402823466e38f) fin = fmaxf(fin, eb);
+                    }
+                });
+                atomicMax(word + 2, __float_as_uint(fin));
                 half_sync(kind);
-                const float need = scale_for(__uint_as_float(*word));
-                const float now = anew ? need : (old >= need ? old : need);  // (an old scale that is NaN is replaced)
-                inv = inverse_scale(now);
-                if (tid == 0) *scale = now;
-                if (!anew && now != old) {
-                    const float ratio = old > 0.f ? old * inv : 0.f;
-                    uint8_t* base = static_cast<uint8_t*>(j.cache[kind]) + block * j.cs_b[kind] + (int64_t)h * j.cs_h[kind];
-                    for (int i = tid; i < j.BS * per_row; i += kAppHalf) {
-                        const int r = i / per_row;
-                        if (ctl->row_token[r] >= 0) continue;
-                        uint4* o = reinterpret_cast<uint4*>(base + (int64_t)r * j.cs_t[kind] + (i - r * per_row) * 16);
-                        const uint4 v = *o;
-                        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-                        uint32_t n[4];
+                largest = word[2];
+            }
+            const float need = scale_for(__uint_as_float(largest));
+            const float now = anew ? need : (old >= need ? old : need);  // (an old scale that is NaN is replaced)
+            inv = inverse_scale(now);
+            if (tid == 0) *scale = now;
+            if (!anew && now != old) {
+                const float ratio = old > 0.f ? old * inv : 0.f;
+                uint8_t* base = static_cast<uint8_t*>(j.cache[kind]) + block * j.cs_b[kind] + (int64_t)h * j.cs_h[kind];
+                for (int i = tid; i < j.BS * per_row; i += kAppHalf) {
+                    const int r = j.by_row.div(i);
+                    if (ctl->row_token[r] >= 0) continue;
+                    uint4* o = reinterpret_cast<uint4*>(base + (int64_t)r * j.cs_t[kind] + (i - r * per_row) * 16);
+                    const uint4 v = *o;
+                    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+                    uint32_t n[4];
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            float f[4];
-                            from_e4m3x4(w[e], f);
+                    for (int e = 0; e < 4; ++e) {
+                        float f[4];
+                        from_e4m3x4(w[e], f);
 #pragma unroll
-                            for (int q = 0; q < 4; ++q) f[q] = ratio > 0.f ? f[q] * ratio : 0.f;
-                            n[e] = to_e4m3x4(f[0], f[1], f[2], f[3]);
-                        }
-                        *o = make_uint4(n[0], n[1], n[2], n[3]);
+                        for (int q = 0; q < 4; ++q) f[q] = ratio > 0.f ? f[q] * ratio : 0.f;
+                        n[e] = to_e4m3x4<false>(f[0], f[1], f[2], f[3]);
                     }
+                    *o = make_uint4(n[0], n[1], n[2], n[3]);
                 }
             }
+            auto put = [&](int row, int ch, const uint2& c0, const uint2& c1) {
+                uint8_t* o = static_cast<uint8_t*>(j.cache[kind]) + block * j.cs_b[kind] + (int64_t)row * j.cs_t[kind] + (int64_t)h * j.cs_h[kind];
+                const ItemPlace at = item_place(TURN, p.ang, ch);
+                if (at.second == at.first + 8) {
+                    *reinterpret_cast<uint4*>(o + at.first) = make_uint4(c0.x, c0.y, c1.x, c1.y);
+                } else {
+                    *reinterpret_cast<uint2*>(o + at.first) = c0;
+                    *reinterpret_cast<uint2*>(o + at.second) = c1;
+                }
+            };
+            if (odd)
+                walk([&](const float (&a)[8], const float (&b)[8], const uint4&, const uint4&, int row, int ch) { put(row, ch, codes8<true>(a, inv), codes8<true>(b, inv)); });
+            else
+                walk([&](const float (&a)[8], const float (&b)[8], const uint4&, const uint4&, int row, int ch) { put(row, ch, codes8<false>(a, inv), codes8<false>(b, inv)); });
+        } else {
+            walk([&](const float (&a)[8], const float (&b)[8], const uint4& wa, const uint4& wb, int row, int ch) {
+                T* o = static_cast<T*>(j.cache[kind]) + block * j.cs_b[kind] + (int64_t)row * j.cs_t[kind] + (int64_t)h * j.cs_h[kind];
+                const ItemPlace at = item_place(TURN, p.ang, ch);
+                uint4 w;
+                w.x = Half2<T>::from_float(a[0], a[1]); w.y = Half2<T>::from_float(a[2], a[3]);
+                w.z = Half2<T>::from_float(a[4], a[5]); w.w = Half2<T>::from_float(a[6], a[7]);
+                *reinterpret_cast<uint4*>(o + at.first) = ch < turn_chunks ? w : wa;
+                w.x = Half2<T>::from_float(b[0], b[1]); w.y = Half2<T>::from_float(b[2], b[3]);
+                w.z = Half2<T>::from_float(b[4], b[5]); w.w = Half2<T>::from_float(b[6], b[7]);
+                *reinterpret_cast<uint4*>(o + at.second) = ch < turn_chunks ? w : wb;
+            });
         }
     }
 }
@@ -299,6 +307,7 @@ __device__ void append_chunk(const AppendParams& p, int64_t cta, float4* cs, App
     const int nh = min(j.heads_per_cta, j.Hkv - h0);
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int64_t n_slots = j.NB * j.BS;
+    const bool small = n_slots <= 0x7fffffff;   // slots divide by multiplication
 
     // candidates: tokens of the chunk whose predecessor in the list lies in another block
     if (tid == 0) { ctl->n_cand = 0; ctl->n_list = 0; }
@@ -315,7 +324,7 @@ __device__ void append_chunk(const AppendParams& p, int64_t cta, float4* cs, App
         }
     }
     const uint32_t votes = __ballot_sync(0xffffffffu, starts);
-    if (lane == 0) ctl->warp_count[warp] = __popc(votes);
+    if (lane == 0 && warp < kAppMaxChunk / 32) ctl->warp_count[warp] = __popc(votes);
     __syncthreads();
     if (starts) {
         int at = __popc(votes & ((1u << lane) - 1));
@@ -331,18 +340,29 @@ __device__ void append_chunk(const AppendParams& p, int64_t cta, float4* cs, App
     const int n_cand = ctl->n_cand;
     if (n_cand == 0) return;
 
-    // the walk: every token of a candidate's block, and whether an earlier token makes another CTA (or candidate) the owner
-    for (int64_t u = tid; u < j.T; u += blockDim.x) {
-        const int64_t s = load_index(j.slots, j.slot_is_int64, u);
-        if (s < 0 || s >= n_slots) continue;
-        const int64_t b = s / j.BS;
-        const uint32_t bit = filter_bit(b);
-        if (!((ctl->filter[bit >> 5] >> (bit & 31)) & 1u)) continue;
-        for (int c = 0; c < n_cand; ++c) {
-            if (ctl->cand_block[c] != b) continue;
-            if (u < ctl->cand_token[c]) { ctl->lead[c] = 0; continue; }
-            const int at = atomicAdd(&ctl->n_list, 1);
-            if (at < kAppList) { ctl->list_cand[at] = c; ctl->list_token[at] = (int)u; }
+    // the walk: every token of a candidate's block, and whether an earlier token makes another CTA (or candidate) the owner;
+    // eight slots at a time, since each is a round trip to L2
+    constexpr int kWalk = 8;
+    for (int64_t u0 = tid; u0 < j.T; u0 += kWalk * 2 * kAppHalf) {
+        int64_t slot[kWalk];
+#pragma unroll
+        for (int k = 0; k < kWalk; ++k) {
+            const int64_t u = u0 + k * 2 * kAppHalf;
+            slot[k] = u < j.T ? load_index(j.slots, j.slot_is_int64, u) : -1;
+        }
+#pragma unroll
+        for (int k = 0; k < kWalk; ++k) {
+            if (slot[k] < 0 || slot[k] >= n_slots) continue;
+            const int64_t b = small ? (int64_t)j.by_block.div((int)slot[k]) : slot[k] / j.BS;
+            const uint32_t bit = filter_bit(b);
+            if (!((ctl->filter[bit >> 5] >> (bit & 31)) & 1u)) continue;
+            const int64_t u = u0 + k * 2 * kAppHalf;
+            for (int c = 0; c < n_cand; ++c) {
+                if (ctl->cand_block[c] != b) continue;
+                if (u < ctl->cand_token[c]) { ctl->lead[c] = 0; continue; }
+                const int at = atomicAdd(&ctl->n_list, 1);
+                if (at < kAppList) { ctl->list_cand[at] = c; ctl->list_token[at] = (int)u; }
+            }
         }
     }
     __syncthreads();
@@ -371,19 +391,28 @@ __device__ void append_chunk(const AppendParams& p, int64_t cta, float4* cs, App
             for (int r0 = 0; r0 < j.BS; r0 += 32) {
                 const bool on = r0 + lane < j.BS && ctl->row_token[r0 + lane] >= 0;
                 const uint32_t m = __ballot_sync(0xffffffffu, on);
-                if (on) ctl->rows[n + __popc(m & ((1u << lane) - 1))] = r0 + lane;
+                if (on) {
+                    const int at = n + __popc(m & ((1u << lane) - 1));
+                    ctl->rows[at] = r0 + lane;
+                    ctl->tokens[at] = ctl->row_token[r0 + lane];
+                }
                 n += __popc(m);
             }
             if (lane == 0) ctl->n_rows = n;
         }
         __syncthreads();
-        store_block<T, CODES>(p, tid / kAppHalf, b, ctl->n_rows, ctl->row_token[0] >= 0, h0, nh, cs, ctl);
+        if (p.ang.inv_freq != nullptr && ctl->n_rows <= kAppTile / j.D) {
+            fill_tile(p, cs, ctl, 0, ctl->n_rows, tid, 2 * kAppHalf);
+            __syncthreads();
+        }
+        if (tid < kAppHalf && p.ang.inv_freq != nullptr) store_block<T, CODES, true>(p, 0, b, ctl->n_rows, ctl->row_token[0] >= 0, h0, nh, cs, ctl);
+        else store_block<T, CODES, false>(p, tid / kAppHalf, b, ctl->n_rows, ctl->row_token[0] >= 0, h0, nh, cs, ctl);
         __syncthreads();
     }
 }
 
 template <typename T, bool CODES>
-__global__ void __launch_bounds__(2 * kAppHalf) kv_append_kernel(const __grid_constant__ AppendParams p)
+__global__ void __launch_bounds__(2 * kAppHalf, 2) kv_append_kernel(const __grid_constant__ AppendParams p)
 {
     extern __shared__ float4 s_dyn[];
     int64_t cta = blockIdx.x;
@@ -397,11 +426,9 @@ __global__ void __launch_bounds__(2 * kAppHalf) kv_append_kernel(const __grid_co
     cta -= n_store;
     const int k = cta < p.rot_ctas[0] ? 0 : 1;
     if (k == 1) cta -= p.rot_ctas[0];
-    if (p.rot_vector[k]) rotate_tile<T>(p.rot[k], p.ang, cta, s_dyn);
-    else rotate_scalar<T>(p.rot[k], p.ang, cta * kRotThreads + threadIdx.x, p.rot_ctas[k] * kRotThreads);
+    if (p.rot_vector[k]) rotate_tile<T, 2 * kAppHalf>(p.rot[k], p.ang, cta, s_dyn);
+    else rotate_scalar<T>(p.rot[k], p.ang, cta * 2 * kAppHalf + threadIdx.x, p.rot_ctas[k] * 2 * kAppHalf);
 }
-
-static_assert(2 * kAppHalf == kRotThreads, "the two roles share a launch");
 
 template <typename T, bool CODES>
 static int launch_append(AppendParams& p, cudaStream_t st)
@@ -432,7 +459,7 @@ static int launch_append(AppendParams& p, cudaStream_t st)
             const size_t need = rotary_smem(r, p.ang.rot);
             if (need > smem) smem = need;
         } else {
-            const int64_t n = (r.T * r.H * (r.D - p.ang.rot / 2) + kRotThreads - 1) / kRotThreads;
+            const int64_t n = (r.T * r.H * (r.D - p.ang.rot / 2) + 2 * kAppHalf - 1) / (2 * kAppHalf);
             p.rot_ctas[k] = n < (int64_t)sms * 8 ? n : (int64_t)sms * 8;
         }
         ctas += p.rot_ctas[k];
@@ -482,7 +509,7 @@ extern "C" int ucmr_kv_append(const void* k, int64_t k_stride_t, int64_t k_strid
     j.cache[0] = k_cache; j.cs_b[0] = kc_stride_block; j.cs_t[0] = kc_stride_t; j.cs_h[0] = kc_stride_h;
     j.cache[1] = v_cache; j.cs_b[1] = vc_stride_block; j.cs_t[1] = vc_stride_t; j.cs_h[1] = vc_stride_h;
     j.scale[0] = k_scale; j.scale[1] = v_scale;
-    j.slots = slot_mapping; j.slot_is_int64 = slot_is_int64; j.T = T; j.NB = NB; j.BS = BS; j.Hkv = Hkv; j.D = D;
+    j.by_row = FastDiv::by((uint32_t)(D / 16)); j.by_block = FastDiv::by((uint32_t)BS); j.slots = slot_mapping; j.slot_is_int64 = slot_is_int64; j.T = T; j.NB = NB; j.BS = BS; j.Hkv = Hkv; j.D = D;
     if (q) {
         RotaryJob& r = p.rot[0];
         r.x = q; r.out = q_out; r.T = T; r.H = Hq; r.D = D;

@@ -20,21 +20,6 @@ inline size_t attn_workspace_bytes(int D)
     return UCMR_WORKSPACE_HEADER_BYTES + kAttnCounterBytes + kAttnPartRows * (D + 2) * sizeof(float);
 }
 
-// Quotients by a fixed divisor (1 .. 2^31 - 1) for numbers below 2^31, without a division: n / d = (hi(m n) + n) >> l with
-// l = ceil(log2 d), m = floor(2^32 (2^l - d) / d) + 1.
-struct FastDiv {
-    uint32_t m, l;
-    static FastDiv by(uint32_t d)
-    {
-        uint32_t l = 0;
-        while (l < 31 && (1u << l) < d) ++l;
-        return FastDiv{(uint32_t)((((1ull << l) - d) << 32) / d + 1), l};
-    }
-#ifdef __CUDACC__
-    __device__ __forceinline__ int div(int n) const { return (int)((__umulhi(m, (uint32_t)n) + (uint32_t)n) >> l); }
-#endif
-};
-
 struct AttnParams {
     const void* q;           // [T, Hq, D]
     int64_t qs_t, qs_h;

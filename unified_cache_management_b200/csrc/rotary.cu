@@ -8,7 +8,7 @@ template <typename T>
 __global__ void __launch_bounds__(kRotThreads) rotary_kernel(const RotaryJob j, const RotaryAngles ang)
 {
     extern __shared__ float4 s_cs[];
-    rotate_tile<T>(j, ang, blockIdx.x, s_cs);
+    rotate_tile<T, kRotThreads>(j, ang, blockIdx.x, s_cs);
 }
 
 template <typename T>

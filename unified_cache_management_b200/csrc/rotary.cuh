@@ -128,6 +128,7 @@ struct RotaryJob {
     int H, D;
     int tok_per_cta, heads_per_cta;  // tile of a CTA
     int head_tiles;
+    FastDiv by_chunks, by_heads;   // divisions by the chunks per head and by heads_per_cta
 };
 
 constexpr int kRotThreads = 256;
@@ -150,6 +151,8 @@ inline void plan_rotary(RotaryJob& j, int rot, int sms)
         j.heads_per_cta = j.H;
     }
     j.head_tiles = (j.H + j.heads_per_cta - 1) / j.heads_per_cta;
+    j.by_chunks = FastDiv::by((uint32_t)chunks);
+    j.by_heads = FastDiv::by((uint32_t)j.heads_per_cta);
 }
 inline int64_t rotary_ctas(const RotaryJob& j)
 {
@@ -167,52 +170,49 @@ inline bool rotary_vector_ok(const RotaryJob& j, int rot)
 
 // HBM-bound: each element is read and written once (2 + 2 bytes).  A CTA computes each (token, pair)'s cosine and sine
 // once, in shared memory, and uses them for all its heads; the first loads are issued before that.
-template <typename T>
+template <typename T, int THREADS>
 __device__ __forceinline__ void rotate_tile(const RotaryJob& j, const RotaryAngles& ang, int64_t cta, float4* cs)
 {
     const int64_t t0 = cta / j.head_tiles * j.tok_per_cta;
     const int h0 = (int)(cta % j.head_tiles) * j.heads_per_cta;
     const int nt = (int)min((int64_t)j.tok_per_cta, j.T - t0), nh = min(j.heads_per_cta, j.H - h0);
     const int chunks = ang.rot / 16, np = ang.rot / 2;
-    const int items = nt * nh * chunks;
-    const T* x = static_cast<const T*>(j.x);
-    T* out = static_cast<T*>(j.out);
-    constexpr int UN = 4;
-    for (int base = 0; base < items; base += UN * kRotThreads) {
+    const int items = nt * j.heads_per_cta * chunks;
+    const T* x = static_cast<const T*>(j.x) + t0 * j.xs_t + (int64_t)h0 * j.xs_h;
+    T* out = static_cast<T*>(j.out) + t0 * j.os_t + (int64_t)h0 * j.os_h;
+    constexpr int UN = 1024 / THREADS;
+    for (int base = 0; base < items; base += 1024) {
         uint4 va[UN], vb[UN];
-        int64_t xo[UN];
         int tok[UN], chn[UN], hd[UN];
 #pragma unroll
         for (int u = 0; u < UN; ++u) {
-            const int i = base + u * kRotThreads + threadIdx.x;
-            if (i < items) {
-                chn[u] = i % chunks;
-                const int r = i / chunks;
-                hd[u] = r % nh;
-                tok[u] = r / nh;
+            const int i = base + u * THREADS + threadIdx.x, r = j.by_chunks.div(i);
+            chn[u] = i - r * chunks;
+            tok[u] = j.by_heads.div(r);
+            hd[u] = i < items ? r - tok[u] * j.heads_per_cta : nh;   // (heads that the last tile lacks are left out)
+            if (hd[u] < nh) {
                 int f, s;
                 pair_offsets(ang.rot, ang.interleaved, chn[u], f, s);
-                xo[u] = (t0 + tok[u]) * j.xs_t + (int64_t)(h0 + hd[u]) * j.xs_h;
-                va[u] = *reinterpret_cast<const uint4*>(x + xo[u] + f);
-                vb[u] = *reinterpret_cast<const uint4*>(x + xo[u] + s);
+                const T* from = x + tok[u] * j.xs_t + hd[u] * j.xs_h;
+                va[u] = *reinterpret_cast<const uint4*>(from + f);
+                vb[u] = *reinterpret_cast<const uint4*>(from + s);
             }
         }
         if (base == 0) {
-            for (int i = threadIdx.x; i < nt * np; i += kRotThreads) {
-                const int row = i / np;
+            for (int i = threadIdx.x; i < nt * np; i += THREADS) {
+                const int row = j.by_chunks.div(i >> 3);
                 fill_cos_sin(cs, ang, load_index(ang.positions, ang.pos_is_int64, t0 + row), row, i - row * np, chunks);
             }
             __syncthreads();
         }
 #pragma unroll
         for (int u = 0; u < UN; ++u) {
-            const int i = base + u * kRotThreads + threadIdx.x;
-            if (i < items) {
+            if (hd[u] < nh) {
                 float a[8], b[8];
                 rotate_pairs<T>(va[u], vb[u], cs + tok[u] * 4 * chunks + chn[u], chunks, ang.interleaved, a, b);
                 int f, s;
                 pair_offsets(ang.rot, ang.interleaved, chn[u], f, s);
-                T* o = out + (t0 + tok[u]) * j.os_t + (int64_t)(h0 + hd[u]) * j.os_h;
+                T* o = out + tok[u] * j.os_t + hd[u] * j.os_h;
                 uint4 w;
                 w.x = Half2<T>::from_float(a[0], a[1]); w.y = Half2<T>::from_float(a[2], a[3]);
                 w.z = Half2<T>::from_float(a[4], a[5]); w.w = Half2<T>::from_float(a[6], a[7]);
@@ -225,12 +225,9 @@ __device__ __forceinline__ void rotate_tile(const RotaryJob& j, const RotaryAngl
     }
     const int rest = (j.D - ang.rot) / 8;  // vectors behind the rotated part: copied, unless they are in place already
     if (rest == 0 || j.x == j.out) return;
-    for (int i = threadIdx.x; i < nt * nh * rest; i += kRotThreads) {
-        const int r = i / rest, e = ang.rot + (i - r * rest) * 8;
-        const int64_t t = t0 + r / nh;
-        const int h = h0 + r % nh;
-        *reinterpret_cast<uint4*>(out + t * j.os_t + (int64_t)h * j.os_h + e) =
-            *reinterpret_cast<const uint4*>(x + t * j.xs_t + (int64_t)h * j.xs_h + e);
+    for (int i = threadIdx.x; i < nt * nh * rest; i += THREADS) {
+        const int r = i / rest, e = ang.rot + (i - r * rest) * 8, t = r / nh, h = r - t * nh;
+        *reinterpret_cast<uint4*>(out + t * j.os_t + h * j.os_h + e) = *reinterpret_cast<const uint4*>(x + t * j.xs_t + h * j.xs_h + e);
     }
 }
 
