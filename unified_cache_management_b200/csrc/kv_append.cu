@@ -19,13 +19,17 @@
 // tokens of its candidates' blocks (a 1024-bit filter in front).  The candidate with the block's first token owns it; if
 // a slot is listed twice, the later token's row is the one that is stored.  So the result does not depend on the order
 // in which CTAs run, whatever the order of the slot list, and no atomic touches global memory.
-// The walk costs T / chunk * head groups * T slot reads out of L2: 134 MB for 32768 tokens in chunks of 128 with two head
-// groups, next to 740 MB of HBM traffic that the call cannot do without.
+// The walk costs T / chunk * head groups * T slot reads out of L2: 67 MB for 32768 tokens in blocks and chunks of 128 with
+// one head group, next to 740 MB of HBM traffic that such a call (8 + 32 heads of 128, e4m3) cannot do without.
 //
-// Keys and values of a candidate go to the two halves of the CTA.  Each half (256 threads) takes the block's rows of one
-// head as a tile of up to 16384 elements held in registers as 16-bit values: load, rotate, largest value, scale, rotate
-// again and store.  Blocks with more elements per head take several tiles; they are walked forwards for the largest value
-// and backwards for the codes, so that the last tile is not read twice.  HBM-bound: 2 bytes read and 1 written per element.
+// Keys and values of a candidate go to the two halves of the CTA (256 threads each), in turn, since keys take longer.  A half
+// goes over the rows of one head of the block twice, first for the largest value, then, out of L2, for the codes.  Cosines
+// and sines of a tile of rows are computed once per block, in shared memory, for all heads.  HBM-bound in principle (2 bytes
+// read and 1 written per element); what it does reach is set by latency and instruction issue: two CTAs of 512 threads fit an
+// SM with 64 registers a thread.  Measured for the call above: 180 us, 84 us of it the queries' rotation (at its floor);
+// 91 us for keys and values without rotation, 136 us with it, where their bytes would take 31 us.  Tried and slower: values
+// held in registers between the passes (234 us in all), halves of 128 threads, one or three CTAs per SM.
+// A decode step of 16 tokens takes 6.5 us on the GPU, bound by latency: walk, filter, rows, two passes.
 #include <cuda_fp8.h>
 
 #include "rotary.cuh"
@@ -60,7 +64,6 @@ struct AppendParams {
     RotaryJob rot[2];       // queries, copy of the rotated keys (T = 0: none)
     int64_t rot_ctas[2];
     int rot_vector[2];
-    int k_vector;           // keys: eight pairs per item
 };
 
 __device__ __forceinline__ void half_sync(int half) { asm volatile("bar.sync %0, %1;" ::"r"(half + 1), "n"(kAppHalf) : "memory"); }
@@ -169,10 +172,10 @@ __device__ __forceinline__ void fill_tile(const AppendParams& p, float4* cs, con
     }
 }
 
-// One half of the CTA stores its kind (0 keys, 1 values) of one block for the CTA's heads.  The cosines of a block that is one
-// tile are there already.
+// One half of the CTA stores the keys (kind 0) or the values (kind 1) of one head of the block in hand.  `turn`: which of the
+// half's heads this is.  The cosines of a block that is one tile are there already.
 template <typename T, bool CODES, bool TURN>
-__device__ __forceinline__ void store_block(const AppendParams& p, int kind, int64_t block, int n_rows, bool anew, int h0, int nh,
+__device__ __forceinline__ void store_head(const AppendParams& p, int half, int kind, int64_t block, int n_rows, bool anew, int h, int turn,
                             float4* cs, AppendCtl* ctl)
 {
     const AppendJob& j = p.store;
@@ -181,120 +184,124 @@ __device__ __forceinline__ void store_block(const AppendParams& p, int kind, int
     const int turn_chunks = TURN ? p.ang.rot / 16 : 0;
     const int tile_rows = kAppTile / j.D;
     const int tiles = (n_rows + tile_rows - 1) / tile_rows;
-    const T* x = static_cast<const T*>(j.x[kind]);
-    int table_of = tiles == 1 ? 0 : -1;  // tile whose cosines are in shared memory
+    const T* x = static_cast<const T*>(j.x[kind]) + (int64_t)h * j.xs_h[kind];
     const uint32_t inf_bits = 0x7f800000u;
-
-    for (int hi = 0; hi < nh; ++hi) {
-        const int h = h0 + hi;
-        float big = 0.f;
-        float inv = 0.f;
-        // f(values, raw values, row, item) for each of the block's items; once for the largest value and once more, out of L2,
-        // for the codes: holding them in registers in between left too few warps to hide the latencies (238 -> see below).
-        auto walk = [&](auto&& f) {
-            for (int tile = 0; tile < tiles; ++tile) {
-                const int r0 = tile * tile_rows, items = min(tile_rows, n_rows - r0) * per_row;
-                if (TURN && table_of != tile) {
-                    half_sync(kind);  // nobody reads the old cosines any more
-                    fill_tile(p, cs, ctl, r0, min(tile_rows, n_rows - r0), tid, kAppHalf);
-                    half_sync(kind);
-                    table_of = tile;
-                }
-#pragma unroll 2
-                for (int i = tid; i < items; i += kAppHalf) {
-                    const int r = j.by_row.div(i), ch = i - r * per_row;
-                    const ItemPlace at = item_place(TURN, p.ang, ch);
-                    const T* src = x + (int64_t)ctl->tokens[r0 + r] * j.xs_t[kind] + (int64_t)h * j.xs_h[kind];
-                    const uint4 va = *reinterpret_cast<const uint4*>(src + at.first), vb = *reinterpret_cast<const uint4*>(src + at.second);
-                    float a[8], b[8];
-                    item_values<T>(va, vb, TURN && ch < turn_chunks, cs + r * 4 * turn_chunks + ch, turn_chunks, p.ang.interleaved, a, b);
-                    f(a, b, va, vb, ctl->rows[r0 + r], ch);
-                }
+    float big = 0.f;
+    float inv = 0.f;
+    // f(values, raw values, row, item) for each of the block's items.  Items in flight per thread: as many as 64 registers hold.
+    constexpr int UNR = TURN ? 2 : 4;
+    auto walk = [&](auto&& f) {
+        for (int tile = 0; tile < tiles; ++tile) {
+            const int r0 = tile * tile_rows, items = min(tile_rows, n_rows - r0) * per_row;
+            if (TURN && tiles > 1) {
+                half_sync(half);  // nobody reads the old cosines any more
+                fill_tile(p, cs, ctl, r0, min(tile_rows, n_rows - r0), tid, kAppHalf);
+                half_sync(half);
             }
-        };
-        if constexpr (CODES) {
+#pragma unroll UNR
+            for (int i = tid; i < items; i += kAppHalf) {
+                const int r = j.by_row.div(i), ch = i - r * per_row;
+                const ItemPlace at = item_place(TURN, p.ang, ch);
+                const T* src = x + (int64_t)ctl->tokens[r0 + r] * j.xs_t[kind];
+                const uint4 va = *reinterpret_cast<const uint4*>(src + at.first), vb = *reinterpret_cast<const uint4*>(src + at.second);
+                float a[8], b[8];
+                item_values<T>(va, vb, TURN && ch < turn_chunks, cs + r * 4 * turn_chunks + ch, turn_chunks, p.ang.interleaved, a, b);
+                f(a, b, va, vb, ctl->rows[r0 + r], ch);
+            }
+        }
+    };
+    if constexpr (CODES) {
+        if constexpr (TURN) {
             walk([&](const float (&a)[8], const float (&b)[8], const uint4&, const uint4&, int, int) {
 #pragma unroll
                 for (int e = 0; e < 8; ++e) big = fmaxf(big, fmaxf(fabsf(a[e]), fabsf(b[e])));   // (NaN has no say)
             });
-            // The half's largest value -> scale (every thread computes the same); old codes are re-rounded if it grows.  The
-            // words were last read two heads ago, on the other side of the previous head's barriers.
-            uint32_t* word = &ctl->big[kind][hi & 1];
-            float* scale = j.scale[kind] + block * j.Hkv + h;
-            const float old = anew ? 0.f : *scale;
-            if (tid == 0) { word[0] = 0; word[2] = 0; }
-            half_sync(kind);  // (also: everybody has read the old scale)
-            const uint32_t m = __reduce_max_sync(0xffffffffu, __float_as_uint(big));
-            if ((tid & 31) == 0) atomicMax(word, m);
-            half_sync(kind);
-            uint32_t largest = word[0];
-            const bool odd = largest >= inf_bits;
-            if (odd) {        // an infinity among them: once more without
-                float fin = 0.f;
-                walk([&](const float (&a)[8], const float (&b)[8], const uint4&, const uint4&, int, int) {
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) {
-                        const float ea = fabsf(a[e]), eb = fabsf(b[e]);
-                        if (ea <= 3.402823466e38f) fin = fmaxf(fin, ea);
-                        if (eb <= 3.402823466e38f) fin = fmaxf(fin, eb);
-                    }
-                });
-                atomicMax(word + 2, __float_as_uint(fin));
-                half_sync(kind);
-                largest = word[2];
-            }
-            const float need = scale_for(__uint_as_float(largest));
-            const float now = anew ? need : (old >= need ? old : need);  // (an old scale that is NaN is replaced)
-            inv = inverse_scale(now);
-            if (tid == 0) *scale = now;
-            if (!anew && now != old) {
-                const float ratio = old > 0.f ? old * inv : 0.f;
-                uint8_t* base = static_cast<uint8_t*>(j.cache[kind]) + block * j.cs_b[kind] + (int64_t)h * j.cs_h[kind];
-                for (int i = tid; i < j.BS * per_row; i += kAppHalf) {
-                    const int r = j.by_row.div(i);
-                    if (ctl->row_token[r] >= 0) continue;
-                    uint4* o = reinterpret_cast<uint4*>(base + (int64_t)r * j.cs_t[kind] + (i - r * per_row) * 16);
-                    const uint4 v = *o;
-                    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-                    uint32_t n[4];
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        float f[4];
-                        from_e4m3x4(w[e], f);
-#pragma unroll
-                        for (int q = 0; q < 4; ++q) f[q] = ratio > 0.f ? f[q] * ratio : 0.f;
-                        n[e] = to_e4m3x4<false>(f[0], f[1], f[2], f[3]);
-                    }
-                    *o = make_uint4(n[0], n[1], n[2], n[3]);
-                }
-            }
-            auto put = [&](int row, int ch, const uint2& c0, const uint2& c1) {
-                uint8_t* o = static_cast<uint8_t*>(j.cache[kind]) + block * j.cs_b[kind] + (int64_t)row * j.cs_t[kind] + (int64_t)h * j.cs_h[kind];
-                const ItemPlace at = item_place(TURN, p.ang, ch);
-                if (at.second == at.first + 8) {
-                    *reinterpret_cast<uint4*>(o + at.first) = make_uint4(c0.x, c0.y, c1.x, c1.y);
-                } else {
-                    *reinterpret_cast<uint2*>(o + at.first) = c0;
-                    *reinterpret_cast<uint2*>(o + at.second) = c1;
-                }
-            };
-            if (odd)
-                walk([&](const float (&a)[8], const float (&b)[8], const uint4&, const uint4&, int row, int ch) { put(row, ch, codes8<true>(a, inv), codes8<true>(b, inv)); });
-            else
-                walk([&](const float (&a)[8], const float (&b)[8], const uint4&, const uint4&, int row, int ch) { put(row, ch, codes8<false>(a, inv), codes8<false>(b, inv)); });
-        } else {
-            walk([&](const float (&a)[8], const float (&b)[8], const uint4& wa, const uint4& wb, int row, int ch) {
-                T* o = static_cast<T*>(j.cache[kind]) + block * j.cs_b[kind] + (int64_t)row * j.cs_t[kind] + (int64_t)h * j.cs_h[kind];
-                const ItemPlace at = item_place(TURN, p.ang, ch);
-                uint4 w;
-                w.x = Half2<T>::from_float(a[0], a[1]); w.y = Half2<T>::from_float(a[2], a[3]);
-                w.z = Half2<T>::from_float(a[4], a[5]); w.w = Half2<T>::from_float(a[6], a[7]);
-                *reinterpret_cast<uint4*>(o + at.first) = ch < turn_chunks ? w : wa;
-                w.x = Half2<T>::from_float(b[0], b[1]); w.y = Half2<T>::from_float(b[2], b[3]);
-                w.z = Half2<T>::from_float(b[4], b[5]); w.w = Half2<T>::from_float(b[6], b[7]);
-                *reinterpret_cast<uint4*>(o + at.second) = ch < turn_chunks ? w : wb;
+        } else {   // two values per instruction
+            uint32_t two = 0;
+            walk([&](const float (&)[8], const float (&)[8], const uint4& va, const uint4& vb, int, int) {
+                two = Half2<T>::abs_max(Half2<T>::abs_max(Half2<T>::abs_max(Half2<T>::abs_max(two, va.x), va.y), va.z), va.w);
+                two = Half2<T>::abs_max(Half2<T>::abs_max(Half2<T>::abs_max(Half2<T>::abs_max(two, vb.x), vb.y), vb.z), vb.w);
             });
+            const float2 f = Half2<T>::to_float(two);
+            big = fmaxf(f.x, f.y);
         }
+        // The half's largest value -> scale (every thread computes the same); old codes are re-rounded if it grows.  The
+        // words were last read two heads ago, on the other side of the previous head's barriers.
+        uint32_t* word = &ctl->big[half][turn & 1];
+        float* scale = j.scale[kind] + block * j.Hkv + h;
+        const float old = anew ? 0.f : *scale;
+        if (tid == 0) { word[0] = 0; word[2] = 0; }
+        half_sync(half);  // (also: everybody has read the old scale)
+        const uint32_t m = __reduce_max_sync(0xffffffffu, __float_as_uint(big));
+        if ((tid & 31) == 0) atomicMax(word, m);
+        half_sync(half);
+        uint32_t largest = word[0];
+        const bool odd = largest >= inf_bits;
+        if (odd) {        // an infinity among them: once more without
+            float fin = 0.f;
+            walk([&](const float (&a)[8], const float (&b)[8], const uint4&, const uint4&, int, int) {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    const float ea = fabsf(a[e]), eb = fabsf(b[e]);
+                    if (ea <= 3.402823466e38f) fin = fmaxf(fin, ea);
+                    if (eb <= 3.402823466e38f) fin = fmaxf(fin, eb);
+                }
+            });
+            atomicMax(word + 2, __float_as_uint(fin));
+            half_sync(half);
+            largest = word[2];
+        }
+        const float need = scale_for(__uint_as_float(largest));
+        const float now = anew ? need : (old >= need ? old : need);  // (an old scale that is NaN is replaced)
+        inv = inverse_scale(now);
+        if (tid == 0) *scale = now;
+        if (!anew && now != old) {
+            const float ratio = old > 0.f ? old * inv : 0.f;
+            uint8_t* base = static_cast<uint8_t*>(j.cache[kind]) + block * j.cs_b[kind] + (int64_t)h * j.cs_h[kind];
+            for (int i = tid; i < j.BS * per_row; i += kAppHalf) {
+                const int r = j.by_row.div(i);
+                if (ctl->row_token[r] >= 0) continue;
+                uint4* o = reinterpret_cast<uint4*>(base + (int64_t)r * j.cs_t[kind] + (i - r * per_row) * 16);
+                const uint4 v = *o;
+                const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+                uint32_t n[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    float f[4];
+                    from_e4m3x4(w[e], f);
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) f[q] = ratio > 0.f ? f[q] * ratio : 0.f;
+                    n[e] = to_e4m3x4<false>(f[0], f[1], f[2], f[3]);
+                }
+                *o = make_uint4(n[0], n[1], n[2], n[3]);
+            }
+        }
+        auto put = [&](int row, int ch, const uint2& c0, const uint2& c1) {
+            uint8_t* o = static_cast<uint8_t*>(j.cache[kind]) + block * j.cs_b[kind] + (int64_t)row * j.cs_t[kind] + (int64_t)h * j.cs_h[kind];
+            const ItemPlace at = item_place(TURN, p.ang, ch);
+            if (at.second == at.first + 8) {
+                *reinterpret_cast<uint4*>(o + at.first) = make_uint4(c0.x, c0.y, c1.x, c1.y);
+            } else {
+                *reinterpret_cast<uint2*>(o + at.first) = c0;
+                *reinterpret_cast<uint2*>(o + at.second) = c1;
+            }
+        };
+        if (odd)
+            walk([&](const float (&a)[8], const float (&b)[8], const uint4&, const uint4&, int row, int ch) { put(row, ch, codes8<true>(a, inv), codes8<true>(b, inv)); });
+        else
+            walk([&](const float (&a)[8], const float (&b)[8], const uint4&, const uint4&, int row, int ch) { put(row, ch, codes8<false>(a, inv), codes8<false>(b, inv)); });
+    } else {
+        walk([&](const float (&a)[8], const float (&b)[8], const uint4& wa, const uint4& wb, int row, int ch) {
+            T* o = static_cast<T*>(j.cache[kind]) + block * j.cs_b[kind] + (int64_t)row * j.cs_t[kind] + (int64_t)h * j.cs_h[kind];
+            const ItemPlace at = item_place(TURN, p.ang, ch);
+            uint4 w;
+            w.x = Half2<T>::from_float(a[0], a[1]); w.y = Half2<T>::from_float(a[2], a[3]);
+            w.z = Half2<T>::from_float(a[4], a[5]); w.w = Half2<T>::from_float(a[6], a[7]);
+            *reinterpret_cast<uint4*>(o + at.first) = ch < turn_chunks ? w : wa;
+            w.x = Half2<T>::from_float(b[0], b[1]); w.y = Half2<T>::from_float(b[2], b[3]);
+            w.z = Half2<T>::from_float(b[4], b[5]); w.w = Half2<T>::from_float(b[6], b[7]);
+            *reinterpret_cast<uint4*>(o + at.second) = ch < turn_chunks ? w : wb;
+        });
     }
 }
 
@@ -405,8 +412,17 @@ __device__ void append_chunk(const AppendParams& p, int64_t cta, float4* cs, App
             fill_tile(p, cs, ctl, 0, ctl->n_rows, tid, 2 * kAppHalf);
             __syncthreads();
         }
-        if (tid < kAppHalf && p.ang.inv_freq != nullptr) store_block<T, CODES, true>(p, 0, b, ctl->n_rows, ctl->row_token[0] >= 0, h0, nh, cs, ctl);
-        else store_block<T, CODES, false>(p, tid / kAppHalf, b, ctl->n_rows, ctl->row_token[0] >= 0, h0, nh, cs, ctl);
+        // Keys take longer than values, by their rotation: the halves take them in turn.  Not where the table of cosines is
+        // filled tile by tile, by the half that holds the keys.
+        const int half = tid / kAppHalf;
+        const bool swap = ctl->n_rows <= kAppTile / j.D;
+        for (int hi = 0; hi < nh; ++hi) {
+            const int kind = swap ? (half + hi) & 1 : half;
+            if (kind == 0 && p.ang.inv_freq != nullptr)
+                store_head<T, CODES, true>(p, half, kind, b, ctl->n_rows, ctl->row_token[0] >= 0, h0 + hi, hi, cs, ctl);
+            else
+                store_head<T, CODES, false>(p, half, kind, b, ctl->n_rows, ctl->row_token[0] >= 0, h0 + hi, hi, cs, ctl);
+        }
         __syncthreads();
     }
 }
@@ -416,7 +432,7 @@ __global__ void __launch_bounds__(2 * kAppHalf, 2) kv_append_kernel(const __grid
 {
     extern __shared__ float4 s_dyn[];
     int64_t cta = blockIdx.x;
-    // the store's CTAs come first: they take longest
+    // the store's CTAs come first: they take longest (spread among the others: 180 -> 253 us)
     const int64_t n_store = (p.store.T + p.store.chunk - 1) / p.store.chunk * p.store.head_tiles;
     if (cta < n_store) {
         AppendCtl* ctl = reinterpret_cast<AppendCtl*>(s_dyn);
@@ -436,13 +452,13 @@ static int launch_append(AppendParams& p, cudaStream_t st)
     AppendJob& j = p.store;
     const int sms = device_sms();
     // Chunk: one token while that leaves at most eight CTAs per SM (a decode step: one owner per CTA), up to 128 tokens
-    // (one walk of the slot list for a whole block of 128).  Heads per CTA: one, doubled while the grid has more than six
-    // CTAs per SM, since every CTA repeats the walk.
+    // (one walk of the slot list for a whole block of 128).  Heads per CTA: one, doubled while the grid has more than three
+    // CTAs per SM, since every CTA repeats the walk and the cosines (measured for the call above: 180 us; up to six 202, twelve 242).
     int64_t chunk = (j.T * j.Hkv + (int64_t)sms * 8 - 1) / ((int64_t)sms * 8);
     j.chunk = (int)(chunk < 1 ? 1 : chunk > kAppMaxChunk ? kAppMaxChunk : chunk);
     const int64_t chunks = (j.T + j.chunk - 1) / j.chunk;
     j.heads_per_cta = 1;
-    while (j.heads_per_cta < j.Hkv && chunks * ((j.Hkv + j.heads_per_cta - 1) / j.heads_per_cta) > (int64_t)sms * 6) j.heads_per_cta *= 2;
+    while (j.heads_per_cta < j.Hkv && chunks * ((j.Hkv + j.heads_per_cta - 1) / j.heads_per_cta) > (int64_t)sms * 3) j.heads_per_cta *= 2;
     j.head_tiles = (j.Hkv + j.heads_per_cta - 1) / j.heads_per_cta;
     int64_t ctas = chunks * j.head_tiles;
     const int tile_rows = kAppTile / j.D < j.BS ? kAppTile / j.D : j.BS;

@@ -57,6 +57,12 @@ template <> struct Half2<__nv_bfloat16> {
         const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
         return reinterpret_cast<const uint32_t&>(h);
     }
+    // larger magnitudes, pair by pair, of a (not negative) and b; a NaN loses
+    static __device__ __forceinline__ uint32_t abs_max(uint32_t a, uint32_t b)
+    {
+        const __nv_bfloat162 h = __hmax2(reinterpret_cast<const __nv_bfloat162&>(a), __habs2(reinterpret_cast<const __nv_bfloat162&>(b)));
+        return reinterpret_cast<const uint32_t&>(h);
+    }
     static __device__ __forceinline__ float to_float1(__nv_bfloat16 v) { return __bfloat162float(v); }
     static __device__ __forceinline__ __nv_bfloat16 from_float1(float v) { return __float2bfloat16_rn(v); }
 };
@@ -65,6 +71,11 @@ template <> struct Half2<__half> {
     static __device__ __forceinline__ uint32_t from_float(float lo, float hi)
     {
         const __half2 h = __floats2half2_rn(lo, hi);
+        return reinterpret_cast<const uint32_t&>(h);
+    }
+    static __device__ __forceinline__ uint32_t abs_max(uint32_t a, uint32_t b)
+    {
+        const __half2 h = __hmax2(reinterpret_cast<const __half2&>(a), __habs2(reinterpret_cast<const __half2&>(b)));
         return reinterpret_cast<const uint32_t&>(h);
     }
     static __device__ __forceinline__ float to_float1(__half v) { return __half2float(v); }
