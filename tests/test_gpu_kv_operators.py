@@ -461,6 +461,171 @@ def test_attention_streams_and_graphs(cuda_device):
         assert int(ws[:2304].count_nonzero()) == 0              # header and counters are back at zero
 
 
+@pytest.mark.parametrize("kind,dtype", [("e4m3", BF), ("e4m3", FP), ("same", BF), ("same", FP)])
+@pytest.mark.parametrize("hq,hkv,d,bs,layout", [(10, 5, 64, 16, "NTHD"), (9, 9, 128, 48, "NHTD"), (12, 12, 64, 7, "NTHD"), (6, 1, 128, 128, "NHTD"),
+                                                (300, 1, 64, 32, "NTHD")])
+def test_attention_many_rows(cuda_device, kind, dtype, hq, hkv, d, bs, layout):
+    """Every pair of types; odd head counts, blocks that end inside a tile of 128 tokens, a block listed twice, lengths around
+    a tile's end, and a batch in which one request has many queries and the others one."""
+    qs = [1, 65, 1, 9, 0, 30] if hq < 300 else [1, 1, 2, 1, 0, 1]
+    c, mq = _case(hq + d, [257, 129, 128, 9, 40, 127], qs, hq, hkv, d, bs, kind, dtype, layout=layout)
+    c["table"][0, 1] = c["table"][0, 0]
+    for causal in (True, False):
+        a = _check(c, mq, causal=causal)
+        b = _attend(c, mq, causal=causal)
+        assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+
+
+@pytest.mark.parametrize("kind", ["e4m3", "same"])
+@pytest.mark.parametrize("hq,hkv,d,bs", [(35, 5, 128, 16), (18, 9, 64, 32), (60, 12, 128, 48), (17, 17, 64, 5), (48, 3, 128, 16)])
+def test_attention_decode_head_counts(cuda_device, kind, hq, hkv, d, bs):
+    """Head counts that do not divide a block of eight warps, groups that are no multiple of four, a block listed twice."""
+    c, mq = _case(hq, [1, 700, 31, 96, 5000], [1] * 5, hq, hkv, d, bs, kind, BF)
+    c["table"][1, 2] = c["table"][1, 0]
+    _check(c, mq)
+
+
+def test_attention_extreme_scales_many_rows(cuda_device):
+    """Scales that differ by more than fp16 holds within a tile, scales of 0 and no power of two, tiles of equal ones.  A weight
+    is counted from 2^(6 - E), 2^E at most twice the largest value scale, in fp16, whose smallest step is 2^-24: each of the
+    n tokens adds at most 448 * 2 * scale * 2^-25 * 2^-6, over a sum of weights of 1 or more (the reference is a score)."""
+    for lo, hi in ((-20, 0), (-90, -60), (60, 90), (-9, 0), (0, 0)):
+        c, mq = _case(52, [400, 90], [33, 20], 8, 2, 64, 16, "e4m3", BF)
+        for i, v in enumerate(torch.linspace(lo, hi, c["v_scale"].shape[0]).round().tolist()):
+            c["v_scale"][i] = 2.0 ** v
+        if lo != hi:
+            c["v_scale"][3] = 0.0
+            c["k_scale"][5] = 0.0
+        if lo == -20:
+            c["k_scale"][6] = 0.37
+        out, lse = _attend(c, mq)
+        want, wlse, room, lroom = R.attention(c["q"], c["k_cache"], c["v_cache"], c["table"], c["seq_lens"], k_scale=c["k_scale"],
+                                              v_scale=c["v_scale"], query_start=c["query_start"])
+        _close(out, want, room + 448.0 * float(c["v_scale"].max()) * 400 * 2.0 ** -30, "out")
+        _close(lse, wlse, lroom, "lse")
+
+
+@pytest.mark.parametrize("kind", ["e4m3", "same"])
+@pytest.mark.parametrize("bs", [16, 24])
+def test_far_blocks(cuda_device, kind, bs):
+    """The last blocks of a cache of more than 2^32 bytes give what they give in a small one, bit for bit."""
+    from unified_cache_management_b200 import ops
+    h, d, dt = 2, 128, E4M3 if kind == "e4m3" else BF
+    qs = [1, 3, 30]
+    c, mq = _case(60, [300, 77, 129], qs, 8, h, d, bs, kind, BF)
+    nb = c["k_cache"].shape[0]
+    many = (1 << 32) // (bs * h * d * dt.itemsize) + 2 * nb
+    if torch.cuda.mem_get_info()[0] < 16 << 30:
+        pytest.skip("needs 16 GB")
+    far = many - nb
+    big = dict(c)
+    for name in ("k_cache", "v_cache"):
+        big[name] = torch.empty((many, bs, h, d), dtype=dt, device="cuda")
+        big[name][far:] = c[name]
+    for name in ("k_scale", "v_scale"):
+        if c[name] is not None:
+            big[name] = torch.ones((many, h), device="cuda")
+            big[name][far:] = c[name]
+    big["table"] = torch.where(c["table"] >= 0, c["table"] + far, c["table"])
+    one = [0, 1, 4]                                            # the requests' first queries, as a decode step
+    for x, y in zip(_attend(big, mq), _attend(c, mq)):
+        assert torch.equal(x, y)
+    for z in (big, c):
+        z["q"], z["query_start"] = z["q"][one].contiguous(), None
+    for x, y in zip(_attend(big, 1), _attend(c, 1)):
+        assert torch.equal(x, y)
+    g = _gen(61)
+    slots = torch.randint(0, nb * bs, (50,), device="cuda", generator=g)
+    k, v = _randn((50, h, d), g, BF, 3.0), _randn((50, h, d), g, BF, 0.1)
+    for z, first in ((big, far * bs), (c, 0)):
+        ops.kv_append(k, v, slots + first, z["k_cache"], z["v_cache"], k_scale=z["k_scale"], v_scale=z["v_scale"])
+    for name in ("k_cache", "v_cache", "k_scale", "v_scale"):
+        if c[name] is not None:
+            assert torch.equal(big[name][far:].view(torch.uint8), c[name].view(torch.uint8)), name
+
+
+def test_append_slots_beyond_31_bits(cuda_device):
+    """Slot numbers above 2^31, in a cache whose rows overlap (block b's row r is row b + r of the memory)."""
+    from unified_cache_management_b200 import ops
+    nb, bs, d = (1 << 21) + 8, 1024, 16
+    mem = [torch.zeros((nb + bs, d), dtype=BF, device="cuda") for _ in range(2)]
+    kc, vc = (m.as_strided((nb, bs, 1, d), (d, d, d, 1)) for m in mem)
+    at = [(nb - 1, 5), (nb - 4, 0), (7, 3), (1 << 20, 1000), (nb - 3, 1)]
+    slots = torch.tensor([b * bs + r for b, r in at] + [nb * bs], device="cuda")
+    x = torch.arange(1.0, 7.0, device="cuda")[:, None, None].expand(6, 1, d).to(BF).contiguous()
+    ops.kv_append(x, -x, slots, kc, vc)
+    for i, (b, r) in enumerate(at[:3]):
+        assert (mem[0][b + r] == i + 1).all() and (mem[1][b + r] == -i - 1).all()
+    assert int(mem[0].count_nonzero()) == 5 * d
+
+
+@pytest.mark.parametrize("kind", ["e4m3", "same"])
+def test_step_captured_and_replayed(cuda_device, kind):
+    """Rotation, append and attention captured into one graph on a stream of its own; replayed with other positions, slots and
+    lengths, it leaves what the eager calls leave."""
+    from unified_cache_management_b200 import ops
+    g = _gen(70)
+    b, hq, h, d, bs, nb = 3, 8, 2, 128, 16, 40
+    kc, vc, ks, vs = _caches(nb, bs, h, d, E4M3 if kind == "e4m3" else BF, g)
+    f, _ = ops.rotary_frequencies(64, device="cuda")
+    table = torch.arange(36, device="cuda").reshape(3, 12).int()
+    qkv = _randn((b, hq + 2 * h, d), g, BF)
+    pos, slot = torch.zeros(b, dtype=torch.int64, device="cuda"), torch.zeros(b, dtype=torch.int64, device="cuda")
+    lens = torch.zeros(b, dtype=torch.int32, device="cuda")
+    ws, out, lse, extra = ops.new_attention_workspace(d, "cuda"), torch.zeros((b, hq, d), dtype=BF, device="cuda"), torch.zeros((b, hq), device="cuda"), torch.zeros_like(qkv)
+
+    def step(kc, vc, ks, vs, ws, out, lse, extra):
+        q, k, v = qkv.split([hq, h, h], 1)
+        ops.rotary(qkv, pos, f, interleaved=True, out=extra)
+        q = ops.kv_append(k, v, slot, kc, vc, k_scale=ks, v_scale=vs, positions=pos, inv_freq=f, q=q)
+        ops.paged_attention(q, kc, vc, table, lens, k_scale=ks, v_scale=vs, workspace=ws, out=out, lse=lse)
+
+    mine = [kc, vc, ks, vs, ws, out, lse, extra]
+    other = [None if x is None else x.clone() for x in mine]
+    slot.fill_(-1)                                             # (nothing is stored while the graph is captured)
+    torch.cuda.synchronize()
+    st, gr = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    with torch.cuda.graph(gr, stream=st):
+        step(*mine)
+    for n in ((1, 30, 16), (2, 31, 17), (3, 0, 18), (140, 192, 19)):
+        lens.copy_(torch.tensor(n, dtype=torch.int32))
+        pos.copy_((lens - 1).long())
+        slot.copy_(torch.where(lens > 0, table[torch.arange(b), (pos // bs).clamp(min=0)].long() * bs + pos % bs, -1))
+        qkv.copy_(_randn(qkv.shape, g, BF))
+        torch.cuda.synchronize()
+        with torch.cuda.stream(st):
+            gr.replay()
+        torch.cuda.synchronize()
+        step(*other)
+        torch.cuda.synchronize()
+        for x, y in zip(mine[:4] + mine[5:], other[:4] + other[5:]):
+            assert x is None or torch.equal(x.view(torch.uint8), y.view(torch.uint8))
+
+
+def test_in_place_and_empty_tables(cuda_device):
+    """Results over their own inputs; requests without a single block."""
+    from unified_cache_management_b200 import ops
+    g = _gen(80)
+    f, _ = ops.rotary_frequencies(64, device="cuda")
+    pos = torch.arange(300, device="cuda")
+    for shape, inter in (((300, 40, 128), False), ((300, 2, 72), True)):
+        x = _randn(shape, g, BF)
+        want = ops.rotary(x, pos, f, interleaved=inter)
+        y = x.clone()
+        ops.rotary(y, pos, f, interleaved=inter, out=y)
+        assert torch.equal(y, want)
+    for qs in ([1, 1], [40, 3]):
+        c, mq = _case(81, [5000, 60], qs, 8, 2, 128, 32, "e4m3", BF)
+        want, _ = _attend(c, mq)
+        q = c["q"].clone()
+        c["q"] = q
+        _attend(c, mq, out=q)
+        assert torch.equal(q, want)
+        c["table"] = torch.empty((2, 0), dtype=torch.int32, device="cuda")
+        out, lse = _attend(c, mq)
+        assert (out == 0).all() and (lse == -math.inf).all()
+
+
 # ---------------------------------------------------------------------------------------------- together
 @pytest.mark.parametrize("kind", ["e4m3", "same"])
 def test_decode_step_from_append_to_attention(cuda_device, kind):

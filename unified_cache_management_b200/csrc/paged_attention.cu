@@ -944,7 +944,7 @@ extern "C" int ucmr_paged_attention(const void* q, int64_t T, int Hq, int D, int
     if (T > 0x7FFFFFFF || NB > 0x7FFFFFFF || (int64_t)max_blocks * BS > 0x7FFFFF00 || (int64_t)max_query_len * (Hq / Hkv) > 0x7FFFFFFF)
         return UCMR_ERR_UNSUPPORTED;
     if (B == 0 || T == 0) return UCMR_OK;
-    if (!q || !k_cache || !v_cache || !block_table || !seq_lens || !out) return UCMR_ERR_BAD_ARG;
+    if (!q || !k_cache || !v_cache || (!block_table && max_blocks > 0) || !seq_lens || !out) return UCMR_ERR_BAD_ARG;
     if (!workspace || workspace_bytes < attn_workspace_bytes(D)) return UCMR_ERR_WORKSPACE;
     const int es = cache_dtype == UCMR_E4M3 ? 1 : 2;
     const uintptr_t bits = reinterpret_cast<uintptr_t>(k_cache) | reinterpret_cast<uintptr_t>(v_cache) | reinterpret_cast<uintptr_t>(workspace);
