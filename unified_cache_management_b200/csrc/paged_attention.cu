@@ -189,6 +189,7 @@ struct DecShared {
     alignas(8) uint64_t landed[kDecWarps][kStages];
     // (a warp's rows take the place of its own ring once its copies have landed)
     static_assert(sizeof(ring[0]) >= NT * 8 * D * 4, "rows do not fit the ring");
+    static_assert(sizeof(ring) >= kDecWarps * 4 * (D + 1) * 4, "the join's sums do not fit the ring");
     float m[kDecWarps][NT * 8], l[kDecWarps][NT * 8];
     float weight[kDecWarps][NT * 8];
     float row_m[kDecWarps][NT * 8], row_l[kDecWarps][NT * 8];
@@ -824,7 +825,7 @@ __global__ void __launch_bounds__(kDecThreads, DecConfig<D, C, NG>::kCtas)
             __syncthreads();
             if (sm.last) {
                 __threadfence();
-                attn_join<D, kSlotRows, kDecWarps, QT>(p, c0, c1, nh * R, warp, lane, [&](int slot_row, int64_t& tok, int& head) {
+                attn_join<D, kSlotRows, kDecWarps, true, QT>(p, c0, c1, nh * R, warp, lane, rows_of(0), [&](int slot_row, int64_t& tok, int& head) {
                     const int h = slot_row / R, r = row0 + slot_row - h * R;
                     tok = s.r.q0 + r / p.G;
                     head = (h0 + h) * p.G + r % p.G;
@@ -881,7 +882,13 @@ static int launch_decode(const AttnParams& p, cudaStream_t st)
     if (e != cudaSuccess) { note_cuda_error(e); (void)cudaGetLastError(); return UCMR_ERR_LAUNCH; }
     const int sms = device_sms(), ctas = (sms < kAttnMaxSms ? sms : kAttnMaxSms) * DecConfig<D, C, NG>::kCtas;
     DecPlan plan;
-    plan.groups = (p.Hkv + kDecWarps - 1) / kDecWarps;
+    // Heads side by side in a CTA: a token's heads lie side by side in memory, but the part that a CTA leaves of an item has
+    // the rows of all its heads, and one CTA adds up an item's parts.  So as many heads, up to four, as leave an item about
+    // ten parts or fewer.  Measured for 8 heads of 128, e4m3, four rows each, in us with 4 | 2 | 1 heads side by side:
+    // 1 request of 131072 tokens 94 | 77 | 68, 4 of 32768 72 | 69 | 72, 16 of 8192 68 | 72 | 74, 200 of 4096 308 | 316 | 341.
+    int heads = 4;
+    while (heads > 1 && (int64_t)ctas * heads > (int64_t)10 * p.B * p.Hkv) heads /= 2;
+    plan.groups = (p.Hkv + heads - 1) / heads;
     plan.heads = (p.Hkv + plan.groups - 1) / plan.groups;
     plan.tokens = kDecWarps / plan.heads;
     // Units of 128 tokens; fewer when even the longest possible batch would not give every CTA two of them.

@@ -95,21 +95,32 @@ template <> struct Out16<__half> {
     }
 };
 
-// Adds up the partial results of one item's CTAs c0 .. c1, in this order, and writes its rows.  CTA c's part lies in slot 2 c,
-// or 2 c + 1 for c0, whose part is the last of its stretch; a slot holds SLOT_ROWS rows of D unnormalised values, then their
-// references, then their sums.  place(row, token, head): where a row of the slot goes, false if nowhere.  A warp takes four
-// rows at a time: its lanes first hold the parts' weights, then D / 32 columns each; eight values are on their way per lane.
-template <int D, int SLOT_ROWS, int WARPS, typename QT, typename Place>
-__device__ __forceinline__ void attn_join(const AttnParams& p, int c0, int c1, int rows, int warp, int lane, Place place)
+// Adds up the partial results of one item's CTAs c0 .. c1 and writes its rows.  CTA c's part lies in slot 2 c, or 2 c + 1 for
+// c0, whose part is the last of its stretch; a slot holds SLOT_ROWS rows of D unnormalised values, then their references,
+// then their sums.  place(row, token, head): where a row of the slot goes, false if nowhere.  A warp takes four rows at a
+// time: its lanes first hold the parts' weights, then D / 32 columns each, of four parts at a time (or two).  `scratch`: WARPS * 4 *
+// (D + 1) floats, so that several warps can share rows when there are few (each takes a run of the parts, and the first adds the
+// others' sums up, in order).  SHARE false: a warp of its own per four rows, no barrier, and less code, where the caller's
+// loops need the instruction cache (prefill of 2 x 4096 tokens: 2110 us, 2485 us with the other form).
+template <int D, int SLOT_ROWS, int WARPS, bool SHARE, typename QT, typename Place>
+__device__ __forceinline__ void attn_join(const AttnParams& p, int c0, int c1, int rows, int warp, int lane, float* scratch, Place place)
 {
-    constexpr int W = D / 32, N = 4;
+    constexpr int W = D / 32, N = 4, kFlight = SHARE ? 4 : 2;
     const float inf = __uint_as_float(0x7f800000u);
     auto slot = [&](int c) { return p.partial + ((int64_t)c * 2 + (c == c0 ? 1 : 0)) * SLOT_ROWS * (D + 2); };
+    int share = 1;                    // warps per four rows
+    if constexpr (SHARE)
+        while (share * 2 * ((rows + N - 1) / N) <= WARPS && share * 8 <= c1 - c0) share *= 2;
+    const int which = SHARE ? warp % share : 0;
 #pragma unroll 1
-    for (int r0 = warp * N; r0 < rows; r0 += WARPS * N) {
+    for (int r0 = SHARE ? warp / share * N : warp * N; r0 < (SHARE && share > 1 ? WARPS / share * N : rows); r0 += SHARE ? WARPS / share * N : WARPS * N) {
+        int64_t tok[N];
+        int head[N];
+        bool live[N];
         float top[N], sum[N], v[N][W];
 #pragma unroll
         for (int n = 0; n < N; ++n) {
+            live[n] = r0 + n < rows && (!SHARE || place(r0 + n, tok[n], head[n]));
             top[n] = -inf;
             sum[n] = 0.f;
 #pragma unroll
@@ -119,26 +130,28 @@ __device__ __forceinline__ void attn_join(const AttnParams& p, int c0, int c1, i
         for (int c = c0 + lane; c <= c1; c += 32)
 #pragma unroll
             for (int n = 0; n < N; ++n)
-                if (r0 + n < rows) top[n] = fmaxf(top[n], __ldcg(slot(c) + SLOT_ROWS * D + r0 + n));
+                if (live[n]) top[n] = fmaxf(top[n], __ldcg(slot(c) + SLOT_ROWS * D + r0 + n));
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1)
 #pragma unroll
             for (int n = 0; n < N; ++n) top[n] = fmaxf(top[n], __shfl_xor_sync(0xffffffffu, top[n], o));
+        const int run = SHARE ? (c1 - c0 + share) / share : c1 - c0 + 1;           // parts per warp
+        const int from = c0 + which * run, to = SHARE ? min(c1, from + run - 1) : c1;
 #pragma unroll 1
-        for (int first = c0; first <= c1; first += 32) {
+        for (int first = from; first <= to; first += 32) {
             const int c = first + lane;
             float weight[N];
 #pragma unroll
             for (int n = 0; n < N; ++n) {
                 weight[n] = 0.f;
-                if (c <= c1 && r0 + n < rows) {
+                if (c <= to && live[n]) {
                     const float m = __ldcg(slot(c) + SLOT_ROWS * D + r0 + n), l = __ldcg(slot(c) + SLOT_ROWS * (D + 1) + r0 + n);
                     weight[n] = m == -inf ? 0.f : exp2_fast(m - top[n]);
                     sum[n] += m == -inf ? l : weight[n] * l;   // (a sum that is NaN stays one)
                 }
             }
-            const int here = min(32, c1 - first + 1);
-#pragma unroll 2
+            const int here = min(32, to - first + 1);
+#pragma unroll kFlight
             for (int k = 0; k < here; ++k) {
                 const float* at = slot(first + k) + r0 * D + lane * W;
                 float x[N][W];
@@ -146,7 +159,7 @@ __device__ __forceinline__ void attn_join(const AttnParams& p, int c0, int c1, i
                 for (int n = 0; n < N; ++n) {
 #pragma unroll
                     for (int i = 0; i < W; ++i) x[n][i] = 0.f;
-                    if (r0 + n >= rows) continue;
+                    if (!live[n]) continue;
                     if constexpr (W == 4) {
                         const float4 y = __ldcg(reinterpret_cast<const float4*>(at + n * D));
                         x[n][0] = y.x; x[n][1] = y.y; x[n][2] = y.z; x[n][3] = y.w;
@@ -168,18 +181,37 @@ __device__ __forceinline__ void attn_join(const AttnParams& p, int c0, int c1, i
         for (int o = 16; o > 0; o >>= 1)
 #pragma unroll
             for (int n = 0; n < N; ++n) sum[n] += __shfl_xor_sync(0xffffffffu, sum[n], o);
+        if (SHARE && share > 1) {     // (the same for the whole CTA, which comes here once)
+            float* mine = scratch + warp * N * (D + 1);
+#pragma unroll
+            for (int n = 0; n < N; ++n) {
+#pragma unroll
+                for (int i = 0; i < W; ++i) mine[n * D + i * 32 + lane] = v[n][i];
+                if (lane == 0) mine[N * D + n] = sum[n];
+            }
+            __syncthreads();
+            if (which != 0) continue;
+#pragma unroll 1
+            for (int w = 1; w < share; ++w) {
+                const float* other = mine + w * N * (D + 1);
+#pragma unroll
+                for (int n = 0; n < N; ++n) {
+#pragma unroll
+                    for (int i = 0; i < W; ++i) v[n][i] += other[n * D + i * 32 + lane];
+                    sum[n] += other[N * D + n];
+                }
+            }
+        }
 #pragma unroll
         for (int n = 0; n < N; ++n) {
-            int64_t tok;
-            int head;
-            if (r0 + n >= rows || !place(r0 + n, tok, head)) continue;
+            if (!live[n] || (!SHARE && !place(r0 + n, tok[n], head[n]))) continue;
             const float inv = sum[n] == 0.f ? 0.f : 1.f / sum[n];
-            QT* out = static_cast<QT*>(p.out) + tok * p.os_t + (int64_t)head * p.os_h + lane * W;
+            QT* out = static_cast<QT*>(p.out) + tok[n] * p.os_t + (int64_t)head[n] * p.os_h + lane * W;
             if constexpr (W == 4)
                 *reinterpret_cast<uint2*>(out) = make_uint2(Out16<QT>::pack(v[n][0] * inv, v[n][1] * inv), Out16<QT>::pack(v[n][2] * inv, v[n][3] * inv));
             else
                 *reinterpret_cast<uint32_t*>(out) = Out16<QT>::pack(v[n][0] * inv, v[n][1] * inv);
-            if (lane == 0 && p.lse != nullptr) p.lse[tok * p.Hq + head] = sum[n] == 0.f ? -inf : (top[n] + log2f(sum[n])) * 0.69314718055994531f;
+            if (lane == 0 && p.lse != nullptr) p.lse[tok[n] * p.Hq + head[n]] = sum[n] == 0.f ? -inf : (top[n] + log2f(sum[n])) * 0.69314718055994531f;
         }
     }
 }

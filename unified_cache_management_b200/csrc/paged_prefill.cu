@@ -848,7 +848,7 @@ __global__ void __launch_bounds__(kThreads, 1) tile_kernel(const __grid_constant
                 bar_sync(1, 256);
                 if (sm.last) {
                     __threadfence();
-                    attn_join<D, 128, 8, QT>(p, c0, c1, min(128, s.n_rows - s.row0), warp, lane, [&](int r, int64_t& to, int& of) {
+                    attn_join<D, 128, 8, false, QT>(p, c0, c1, min(128, s.n_rows - s.row0), warp, lane, nullptr, [&](int r, int64_t& to, int& of) {
                         to = s.q0 + (s.row0 + r) / p.G;
                         of = s.h * p.G + (s.row0 + r) % p.G;
                         return true;
@@ -1160,7 +1160,7 @@ __global__ void __launch_bounds__(kThreads, 1) tile_kernel(const __grid_constant
                     const TileSlot& slot = sm.tile[tile % kTileSlots];
                     more = !slot.end;
                     if (C == kE4m3 && more) {
-#pragma unroll 1
+#pragma unroll
                         for (int at = lane; at < kTok; at += 32) {
                             const int blk = slot.block[at];
                             if (blk < 0) continue;
@@ -1181,7 +1181,7 @@ __global__ void __launch_bounds__(kThreads, 1) tile_kernel(const __grid_constant
                         for (int kind = 0; kind < 2; ++kind) {
                             const float* of = sm.scale[t & 1][kind];
                             uint32_t lo = 0xffffffffu, hi = 0, odd = 0, zero = 0;
-#pragma unroll 1
+#pragma unroll
                             for (int at = lane; at < kTok; at += 32) {
                                 if (slot.block[at] < 0) continue;
                                 const uint32_t b = __float_as_uint(of[at]);
@@ -1204,7 +1204,7 @@ __global__ void __launch_bounds__(kThreads, 1) tile_kernel(const __grid_constant
                                 slot.folds[kind] = fold;
                             }
                             if (fold || general) {
-#pragma unroll 1
+#pragma unroll
                                 for (int at = lane; at < kTok; at += 32) {
                                     const float v = slot.block[at] < 0 ? 0.f : of[at];
                                     // 2^-d with d up to 15 (the last one subnormal), 0 for 0, twice in fp16
@@ -1216,7 +1216,7 @@ __global__ void __launch_bounds__(kThreads, 1) tile_kernel(const __grid_constant
                         }
                     }
                     const int bad = slot.bad;
-#pragma unroll 1
+#pragma unroll
                     for (int k = 0; k < 4; ++k) {    // (behind the end the limits hide the tokens)
                         const uint32_t votes = bad ? __ballot_sync(0xffffffffu, slot.block[k * 32 + lane] >= 0) : 0xffffffffu;
                         if (lane == 0) mt.valid[k] = votes;
