@@ -1,31 +1,42 @@
 // Attention over the paged KV cache (sm_100a): out = softmax(scale * q k^T) v over the tokens of the blocks that a table
-// lists, for decode steps, speculative verification and short prefills.  Cache of 16-bit values, or of e4m3 codes with a
-// scale per (block, kv head).
+// lists, for up to 16 rows per (request, kv head): decode steps and short verifications.  Calls with more rows go to
+// paged_prefill.cu (verification of 4 tokens with 8 query heads per kv head, 32 rows: 138 us there, 318 us here in two row
+// tiles; 16 rows, 16 requests of 8192 tokens: 131 us here, 168 us there).  Cache of 16-bit values, or of e4m3 codes with a scale
+// per (block, kv head).
 //
-// Work.  An item is (request, row tile, kv head): the G query heads of a kv head times the request's query tokens give
-// rows; NT * 8 of them share one pass over the keys.  Its tokens are cut into units of 128.  All units of all items form
-// one line, which is divided evenly over the CTAs (two per SM): ragged batches balance, and one long request is split
-// over the whole GPU.  A CTA that has only a part of an item leaves (max, sum, unnormalised rows) in its slot of the
-// workspace; the last of an item's CTAs to arrive adds the parts up, in the order of the tokens: results do not depend
-// on timing.  HBM-bound for up to 16 rows: the keys and values are read once.
+// Work.  The G query heads of a kv head times the request's query tokens are rows; 4, 8 or 16 of them (a row tile) share one
+// pass over the keys.  An item is (request, row tile, up to four kv heads side by side); its tokens are cut into units.  All
+// units of all items form one line, which is divided evenly over the CTAs (two per SM where registers and shared memory
+// allow it): ragged batches balance, and one long request is split over the whole GPU.  A CTA that has only a part of an item
+// leaves (max, sum, unnormalised rows) in its slot of the workspace; the last of an item's CTAs to arrive adds the parts up,
+// in the order of the tokens: results do not depend on timing.
 //
-// A unit is eight warps times 16 tokens, and the warps do not wait for one another.  Each has a ring of stages in shared
-// memory that its own lanes fill with 16-byte asynchronous copies; a lane reads back only what it copied itself, so a
-// stage needs no barrier, and block ids, scales and tails are handled per token: any block size, any strides.
-//   S^T = K Q^T: tokens are the 16 rows of mma.m16n8k16, query rows its 8 columns.  The order in which the products run
-//     over the head dimension is free, so each lane takes 16 consecutive bytes of a key (4 lanes per key), converts them
-//     and has its fragments; the queries are read in the same order.
+// Eight warps, each with one of the item's heads and every n-th group of 16 tokens; they do not wait for one another until
+// the item ends.  Each has a ring of stages of 16 tokens in shared memory.  Where a block holds a multiple of 16 tokens, one
+// thread has the copy engine fetch a stage's keys and values (boxes of 16 tokens of a head; a mbarrier tells when they are
+// there): 16 x 131072 tokens 952 -> 710 us against copies by all lanes, which were bound by their instructions.  Otherwise all
+// lanes copy, 16 bytes at a time, with block ids and tails per token: any block size, any strides.
+//   S^T = K Q^T: tokens are the 16 rows of the matrix instruction, query rows its 8 columns.  The order in which the products
+//     run over the head dimension is free, so each lane takes 16 consecutive bytes of a key (4 lanes per key), and the
+//     queries are read in the same order.
 //   O^T += V^T P^T: the head dimension is the 16 rows, again in a free order: each lane takes D/8 consecutive values of four
 //     tokens, and interleaves the tokens two by two for its fragments.  P^T is S^T's fragment, transposed by movmatrix.
-// mma.sync serves here because the rows are few: 16 x 8 tiles waste nothing, and the tensor work is a fifth of what the
-// legacy path can do while the memory system is saturated.
+// mma.sync serves here because the rows are few: 16 x 8 tiles waste little, where a tile of the tensor memory has 128 rows.
 //
-// Numerics.  e4m3 codes become fp16 exactly; queries become fp16 after a power of two per row has brought them to at most
-// 2 (bf16 -> fp16 is then exact but for values below 2^-24 of the row's largest).  Scores, softmax and rows are float32; the key scale and the softmax scale are applied to
-// the float32 score.  The probability that multiplies V is rounded to fp16 (half a step: 2^-11) with the value scale
-// folded in, counted from 2^(14 - E), E the exponent of the largest value scale so far: the largest product is 2^14, so
-// probabilities down to 2^-28 of the largest keep all bits and those below 2^-39 are dropped.  A bf16 cache uses bf16 operands
-// (probabilities rounded by 2^-8), an fp16 cache fp16 ones.
+// Numerics.  e4m3 codes against bf16 queries: the query row, after a power of two has brought its largest value to 448 or
+// less, is the sum of two e4m3 values (4 + 4 of bf16's 8 significant bits): exactly for elements down to 2^-9 of the row's
+// largest, and to half of 2^-9, which is 2^-17 of the row's largest, for smaller ones.  So keys are multiplied as the codes
+// they are, by two columns per query row, m16n8k32, whose sums are float32.  Against fp16 queries (11 bits) codes become fp16,
+// exactly, and so do the queries after a power of two per row.  Scores, softmax and rows are float32; the key scale and the
+// softmax scale are applied to the float32 score.  The probability that multiplies V is rounded to fp16 (half a step: 2^-11)
+// with the value scale folded in, counted from 2^(14 - E), E the exponent of the largest value scale so far: the largest
+// product is 2^14, so probabilities down to 2^-28 of the largest keep all bits and those below 2^-39 are dropped.  A bf16
+// cache uses bf16 operands (probabilities rounded by 2^-8), an fp16 cache fp16 ones.
+//
+// What bounds it: HBM for 4 rows and long contexts (16 x 131072 tokens, 8 heads of 128, e4m3: 730 us, 5.9 TB/s; 64 x 4096
+// tokens in bf16: 180 us, 6.0 TB/s); for 8 and 16 rows of e4m3 the issue of instructions (940 and 1400 us for the former).  Calls
+// of some 10 us of traffic pay 20 to 30 us for the launch, the line, the first copies and the join (16 x 8192 tokens: 70 us
+// for 268 MB).
 #include <cuda.h>
 
 #include "paged_attention.cuh"
@@ -495,71 +506,55 @@ __global__ void __launch_bounds__(kDecThreads, DecConfig<D, C, NG>::kCtas)
                 }
                 phases ^= 1u << slot;
             }
-            constexpr int kSub = 1;
-            const unsigned char* st[kSub] = {&sm.ring[warp][slot][0]};
-            uint32_t mask[kSub] = {mark};
+            const unsigned char* st = &sm.ring[warp][slot][0];
             const bool whole = (mark & 0xffffu) == 0xffffu;
             const int tok0 = tok_at(i);
 
             // scores of the tokens token(g) and token(g) + 8
-            float sc[kSub][kQRegs][4];
+            float sc[kQRegs][4];
 #pragma unroll
-            for (int u = 0; u < kSub; ++u)
-#pragma unroll
-                for (int nt = 0; nt < kQRegs; ++nt) sc[u][nt][0] = sc[u][nt][1] = sc[u][nt][2] = sc[u][nt][3] = 0.f;
+            for (int nt = 0; nt < kQRegs; ++nt) sc[nt][0] = sc[nt][1] = sc[nt][2] = sc[nt][3] = 0.f;
 #pragma unroll
             for (int c = 0; c < Sh::kKPieces; ++c) {
-                uint32_t wl[kSub][4], wh[kSub][4];
-#pragma unroll
-                for (int u = 0; u < kSub; ++u) {
-                    const uint4 lo = *reinterpret_cast<const uint4*>(st[u] + Sh::at(mine, c * 4 + t));
-                    const uint4 hi = *reinterpret_cast<const uint4*>(st[u] + Sh::at(mine + 8, c * 4 + t));
-                    wl[u][0] = lo.x; wl[u][1] = lo.y; wl[u][2] = lo.z; wl[u][3] = lo.w;
-                    wh[u][0] = hi.x; wh[u][1] = hi.y; wh[u][2] = hi.z; wh[u][3] = hi.w;
-                }
+                uint32_t wl[4], wh[4];
+                const uint4 lo = *reinterpret_cast<const uint4*>(st + Sh::at(mine, c * 4 + t));
+                const uint4 hi = *reinterpret_cast<const uint4*>(st + Sh::at(mine + 8, c * 4 + t));
+                wl[0] = lo.x; wl[1] = lo.y; wl[2] = lo.z; wl[3] = lo.w;
+                wh[0] = hi.x; wh[1] = hi.y; wh[2] = hi.z; wh[3] = hi.w;
                 if constexpr (kQ8) {
 #pragma unroll
                     for (int w = 0; w < 2; ++w)
 #pragma unroll
-                        for (int u = 0; u < kSub; ++u)
-#pragma unroll
-                            for (int nt = 0; nt < kQRegs; ++nt)
-                                mma_16832(sc[u][nt], wl[u][2 * w], wh[u][2 * w], wl[u][2 * w + 1], wh[u][2 * w + 1],
-                                          qf[nt][c * 2 + w][0], qf[nt][c * 2 + w][1]);
+                        for (int nt = 0; nt < kQRegs; ++nt)
+                            mma_16832(sc[nt], wl[2 * w], wh[2 * w], wl[2 * w + 1], wh[2 * w + 1],
+                                      qf[nt][c * 2 + w][0], qf[nt][c * 2 + w][1]);
                 } else if constexpr (C == kE4m3) {
 #pragma unroll
-                    for (int w = 0; w < 4; ++w)
+                    for (int w = 0; w < 4; ++w) {
+                        const uint32_t a0 = e4m3x2_to_f16x2(wl[w]), a2 = e4m3x2_to_f16x2(wl[w] >> 16);
+                        const uint32_t a1 = e4m3x2_to_f16x2(wh[w]), a3 = e4m3x2_to_f16x2(wh[w] >> 16);
 #pragma unroll
-                        for (int u = 0; u < kSub; ++u) {
-                            const uint32_t a0 = e4m3x2_to_f16x2(wl[u][w]), a2 = e4m3x2_to_f16x2(wl[u][w] >> 16);
-                            const uint32_t a1 = e4m3x2_to_f16x2(wh[u][w]), a3 = e4m3x2_to_f16x2(wh[u][w] >> 16);
-#pragma unroll
-                            for (int nt = 0; nt < NT; ++nt)
-                                mma_16816<C>(sc[u][nt], a0, a1, a2, a3, qf[nt][c * 4 + w][0], qf[nt][c * 4 + w][1]);
-                        }
+                        for (int nt = 0; nt < NT; ++nt)
+                            mma_16816<C>(sc[nt], a0, a1, a2, a3, qf[nt][c * 4 + w][0], qf[nt][c * 4 + w][1]);
+                    }
                 } else {
 #pragma unroll
                     for (int w = 0; w < 2; ++w)
 #pragma unroll
-                        for (int u = 0; u < kSub; ++u)
-#pragma unroll
-                            for (int nt = 0; nt < NT; ++nt)
-                                mma_16816<C>(sc[u][nt], wl[u][2 * w], wh[u][2 * w], wl[u][2 * w + 1], wh[u][2 * w + 1],
-                                             qf[nt][c * 2 + w][0], qf[nt][c * 2 + w][1]);
+                        for (int nt = 0; nt < NT; ++nt)
+                            mma_16816<C>(sc[nt], wl[2 * w], wh[2 * w], wl[2 * w + 1], wh[2 * w + 1],
+                                         qf[nt][c * 2 + w][0], qf[nt][c * 2 + w][1]);
                 }
             }
-            float vfac[kSub][2], kfac[kSub][2];
+            float vfac[2], kfac[2];
             float vdown = 1.f;
             if constexpr (C == kE4m3) {
                 uint32_t big = 0;
-#pragma unroll
-                for (int u = 0; u < kSub; ++u) {
-                    const float* f = sm.scale[warp][slot];
-                    const int one = TMA ? 0 : mine, two = TMA ? 0 : mine + 8;    // (one scale for all 16 tokens of a block)
-                    kfac[u][0] = f[one]; kfac[u][1] = f[two];
-                    vfac[u][0] = f[16 + one]; vfac[u][1] = f[16 + two];
-                    big = max(big, max(__float_as_uint(fabsf(vfac[u][0])), __float_as_uint(fabsf(vfac[u][1]))));
-                }
+                const float* f = sm.scale[warp][slot];
+                const int one = TMA ? 0 : mine, two = TMA ? 0 : mine + 8;    // (one scale for all 16 tokens of a block)
+                kfac[0] = f[one]; kfac[1] = f[two];
+                vfac[0] = f[16 + one]; vfac[1] = f[16 + two];
+                big = max(big, max(__float_as_uint(fabsf(vfac[0])), __float_as_uint(fabsf(vfac[1]))));
                 if (!TMA) big = __reduce_max_sync(0xffffffffu, big);   // (the same in all lanes otherwise)
                 const int e = max(-100, min(128, (int)(big >> 23) - 126));  // every scale is below 2^e
                 if (e > vexp) {
@@ -567,46 +562,39 @@ __global__ void __launch_bounds__(kDecThreads, DecConfig<D, C, NG>::kCtas)
                     vexp = e;
                     vup = exp2_fast(kShift - (float)vexp);  // a power of two
                 }
-#pragma unroll
-                for (int u = 0; u < kSub; ++u) { vfac[u][0] *= vup; vfac[u][1] *= vup; }
+                vfac[0] *= vup; vfac[1] *= vup;
             } else {
-#pragma unroll
-                for (int u = 0; u < kSub; ++u) { vfac[u][0] = vfac[u][1] = C == kBf16 ? 1.f : 16384.f; kfac[u][0] = kfac[u][1] = 1.f; }
+                vfac[0] = vfac[1] = C == kBf16 ? 1.f : 16384.f; kfac[0] = kfac[1] = 1.f;
             }
-            const bool edge = !whole || tok0 + kSub * 16 > min_limit;
+            const bool edge = !whole || tok0 + 16 > min_limit;
             bool grown = vdown != 1.f;
             float alpha[NT][2];
-            uint32_t pf[kSub][NT][2];
+            uint32_t pf[NT][2];
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
                 constexpr int kLast = NG - 2 * (NT - 1);     // rows t and, but for the last of an odd number of fours, t + 4
                 const int cols = nt == NT - 1 ? kLast : 2;
-                float x[kSub][4];
+                float x[4];
 #pragma unroll
-                for (int u = 0; u < kSub; ++u)
-#pragma unroll
-                    for (int c = 0; c < 4; ++c) {
-                        x[u][c] = 0.f;
-                        if ((c & 1) >= cols) continue;
-                        float v;
-                        if constexpr (kQ8) {
-                            const int group = nt * 2 + (c & 1) < kQRegs ? nt * 2 + (c & 1) : 0;
-                            v = sc[u][group][c & 2] + sc[u][group][(c & 2) + 1];
-                        } else {
-                            v = sc[u][nt < kQRegs ? nt : 0][c];
-                        }
-                        x[u][c] = v * (kfac[u][c >> 1] * qmul[nt][c & 1]);
-                        if (edge) {
-                            const int tk = mine + 8 * (c >> 1);
-                            if (!((mask[u] >> tk) & 1u) || tok0 + u * 16 + tk >= limit[nt][c & 1]) x[u][c] = -inf;
-                        }
+                for (int c = 0; c < 4; ++c) {
+                    x[c] = 0.f;
+                    if ((c & 1) >= cols) continue;
+                    float v;
+                    if constexpr (kQ8) {
+                        const int group = nt * 2 + (c & 1) < kQRegs ? nt * 2 + (c & 1) : 0;
+                        v = sc[group][c & 2] + sc[group][(c & 2) + 1];
+                    } else {
+                        v = sc[nt < kQRegs ? nt : 0][c];
                     }
+                    x[c] = v * (kfac[c >> 1] * qmul[nt][c & 1]);
+                    if (edge) {
+                        const int tk = mine + 8 * (c >> 1);
+                        if (!((mark >> tk) & 1u) || tok0 + tk >= limit[nt][c & 1]) x[c] = -inf;
+                    }
+                }
                 float top[2];
 #pragma unroll
-                for (int c = 0; c < 2; ++c) {
-                    top[c] = fmaxf(x[0][c], x[0][c + 2]);
-                    if (kSub == 2) top[c] = fmaxf(top[c], fmaxf(x[kSub - 1][c], x[kSub - 1][c + 2]));
-                }
+                for (int c = 0; c < 2; ++c) top[c] = fmaxf(x[c], x[c + 2]);
 #pragma unroll
                 for (int w = 4; w < 32; w <<= 1)
 #pragma unroll
@@ -622,21 +610,13 @@ __global__ void __launch_bounds__(kDecThreads, DecConfig<D, C, NG>::kCtas)
                         grown = true;
                     }
                     const float ref = m[nt][c] == -inf ? 0.f : m[nt][c];
-                    float sum = 0.f;
-#pragma unroll
-                    for (int u = 0; u < kSub; ++u) {
-                        const float p0 = exp2_fast(x[u][c] - ref), p1 = exp2_fast(x[u][c + 2] - ref);
-                        sum += p0 + p1;
-                        x[u][c] = p0 * vfac[u][0];
-                        x[u][c + 2] = p1 * vfac[u][1];
-                    }
-                    l[nt][c] = l[nt][c] * alpha[nt][c] + sum;
+                    const float p0 = exp2_fast(x[c] - ref), p1 = exp2_fast(x[c + 2] - ref);
+                    x[c] = p0 * vfac[0];
+                    x[c + 2] = p1 * vfac[1];
+                    l[nt][c] = l[nt][c] * alpha[nt][c] + (p0 + p1);
                 }
-#pragma unroll
-                for (int u = 0; u < kSub; ++u) {
-                    pf[u][nt][0] = transpose_8x8(pack_p<C == kBf16 ? kBf16 : kF16>(x[u][0], x[u][1]));
-                    pf[u][nt][1] = transpose_8x8(pack_p<C == kBf16 ? kBf16 : kF16>(x[u][2], x[u][3]));
-                }
+                pf[nt][0] = transpose_8x8(pack_p<C == kBf16 ? kBf16 : kF16>(x[0], x[1]));
+                pf[nt][1] = transpose_8x8(pack_p<C == kBf16 ? kBf16 : kF16>(x[2], x[3]));
             }
             if (__any_sync(0xffffffffu, grown)) {
 #pragma unroll
@@ -651,95 +631,91 @@ __global__ void __launch_bounds__(kDecThreads, DecConfig<D, C, NG>::kCtas)
             }
             // values: D/8 consecutive ones of the tokens that are rows 2t, 2t+1, 2t+8, 2t+9 of the products
             constexpr int W = Sh::kVBytes / 4;
+            const unsigned char* sv = st + Sh::kTile;
+            const int part = Sh::eighth(g);
+            auto value_at = [&](int tk) { return sv + Sh::at(tk, part * Sh::kVBytes / 16) + (part * Sh::kVBytes) % 16; };
+            uint32_t vw[4][W];
 #pragma unroll
-            for (int u = 0; u < kSub; ++u) {
-                const unsigned char* sv = st[u] + Sh::kTile;
-                const int part = Sh::eighth(g);
-                auto value_at = [&](int tk) { return sv + Sh::at(tk, part * Sh::kVBytes / 16) + (part * Sh::kVBytes) % 16; };
-                uint32_t vw[4][W];
+            for (int k = 0; k < 4; ++k) {
+                const int tk = Sh::token(2 * t + (k & 1)) + 8 * (k >> 1);
+                if constexpr (Sh::kVBytes >= 16) {
 #pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    const int tk = Sh::token(2 * t + (k & 1)) + 8 * (k >> 1);
-                    if constexpr (Sh::kVBytes >= 16) {
-#pragma unroll
-                        for (int c = 0; c < Sh::kVBytes / 16; ++c) {
-                            const uint4 v = *reinterpret_cast<const uint4*>(sv + Sh::at(tk, part * (Sh::kVBytes / 16) + c));
-                            vw[k][c * 4] = v.x; vw[k][c * 4 + 1] = v.y; vw[k][c * 4 + 2] = v.z; vw[k][c * 4 + 3] = v.w;
-                        }
-                    } else {
-                        const uint2 v = *reinterpret_cast<const uint2*>(value_at(tk));
-                        vw[k][0] = v.x;
-                        vw[k][1] = v.y;
+                    for (int c = 0; c < Sh::kVBytes / 16; ++c) {
+                        const uint4 v = *reinterpret_cast<const uint4*>(sv + Sh::at(tk, part * (Sh::kVBytes / 16) + c));
+                        vw[k][c * 4] = v.x; vw[k][c * 4 + 1] = v.y; vw[k][c * 4 + 2] = v.z; vw[k][c * 4 + 3] = v.w;
                     }
+                } else {
+                    const uint2 v = *reinterpret_cast<const uint2*>(value_at(tk));
+                    vw[k][0] = v.x;
+                    vw[k][1] = v.y;
                 }
-                const int tok16 = tok0 + u * 16;
-                if (edge) {
-                    // Some rows, or all, do not see some of these tokens: a value that is not finite must not reach them as
-                    // 0 * NaN.  It is taken out of the product and added by itself to the rows that see it.
-                    bool odd = false;
+            }
+            if (edge) {
+                // Some rows, or all, do not see some of these tokens: a value that is not finite must not reach them as
+                // 0 * NaN.  It is taken out of the product and added by itself to the rows that see it.
+                bool odd = false;
 #pragma unroll
-                    for (int k = 0; k < 4; ++k)
+                for (int k = 0; k < 4; ++k)
 #pragma unroll
-                        for (int w = 0; w < W; ++w) {
-                            if constexpr (C == kE4m3) {
+                    for (int w = 0; w < W; ++w) {
+                        if constexpr (C == kE4m3) {
 #pragma unroll
-                                for (int e = 0; e < 4; ++e)
-                                    if (((vw[k][w] >> (8 * e)) & 0x7fu) == 0x7fu) { vw[k][w] &= ~(0xffu << (8 * e)); odd = true; }
-                            } else {
-                                constexpr uint32_t kExp = C == kBf16 ? 0x7f80u : 0x7c00u;
+                            for (int e = 0; e < 4; ++e)
+                                if (((vw[k][w] >> (8 * e)) & 0x7fu) == 0x7fu) { vw[k][w] &= ~(0xffu << (8 * e)); odd = true; }
+                        } else {
+                            constexpr uint32_t kExp = C == kBf16 ? 0x7f80u : 0x7c00u;
 #pragma unroll
-                                for (int e = 0; e < 2; ++e)
-                                    if (((vw[k][w] >> (16 * e)) & kExp) == kExp) { vw[k][w] &= ~(0xffffu << (16 * e)); odd = true; }
-                            }
+                            for (int e = 0; e < 2; ++e)
+                                if (((vw[k][w] >> (16 * e)) & kExp) == kExp) { vw[k][w] &= ~(0xffffu << (16 * e)); odd = true; }
                         }
-                    if (__any_sync(0xffffffffu, odd)) {
+                    }
+                if (__any_sync(0xffffffffu, odd)) {
 #pragma unroll 1
-                        for (int tk = 0; tk < 16; ++tk) {
-                            if (!((mask[u] >> tk) & 1u)) continue;
+                    for (int tk = 0; tk < 16; ++tk) {
+                        if (!((mark >> tk) & 1u)) continue;
 #pragma unroll
-                            for (int d = 0; d < D / 8; ++d) {
-                                const int byte = d * Sh::kEs;
-                                const unsigned char* at;
-                                if constexpr (Sh::kVBytes >= 16) at = sv + Sh::at(tk, part * (Sh::kVBytes / 16) + byte / 16) + byte % 16;
-                                else at = value_at(tk) + byte;
-                                float v = 0.f;
-                                if constexpr (C == kE4m3) {
-                                    if ((*at & 0x7fu) == 0x7fu) v = __uint_as_float(0x7fffffffu);
-                                } else {
-                                    const float x = unpack_16(*reinterpret_cast<const uint16_t*>(at), 0, C == kBf16);
-                                    if (!(fabsf(x) <= 3.402823466e38f)) v = x;
-                                }
-                                if (v == 0.f) continue;
-#pragma unroll
-                                for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-                                    for (int c = 0; c < 2; ++c)
-                                        if (tok16 + tk < limit[nt][c]) o[nt][d / 2][(d & 1) * 2 + c] += v;
+                        for (int d = 0; d < D / 8; ++d) {
+                            const int byte = d * Sh::kEs;
+                            const unsigned char* at;
+                            if constexpr (Sh::kVBytes >= 16) at = sv + Sh::at(tk, part * (Sh::kVBytes / 16) + byte / 16) + byte % 16;
+                            else at = value_at(tk) + byte;
+                            float v = 0.f;
+                            if constexpr (C == kE4m3) {
+                                if ((*at & 0x7fu) == 0x7fu) v = __uint_as_float(0x7fffffffu);
+                            } else {
+                                const float x = unpack_16(*reinterpret_cast<const uint16_t*>(at), 0, C == kBf16);
+                                if (!(fabsf(x) <= 3.402823466e38f)) v = x;
                             }
+                            if (v == 0.f) continue;
+#pragma unroll
+                            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                                for (int c = 0; c < 2; ++c)
+                                    if (tok0 + tk < limit[nt][c]) o[nt][d / 2][(d & 1) * 2 + c] += v;
                         }
                     }
                 }
+            }
 #pragma unroll
-                for (int w = 0; w < W; ++w) {
-                    if constexpr (C == kE4m3) {
-                        // bytes of two tokens side by side: (token 0, token 1) of values 4w, 4w+1 | 4w+2, 4w+3
-                        const uint32_t x0 = __byte_perm(vw[0][w], vw[1][w], 0x5140), x1 = __byte_perm(vw[0][w], vw[1][w], 0x7362);
-                        const uint32_t y0 = __byte_perm(vw[2][w], vw[3][w], 0x5140), y1 = __byte_perm(vw[2][w], vw[3][w], 0x7362);
-                        const uint32_t a0 = e4m3x2_to_f16x2(x0), a1 = e4m3x2_to_f16x2(x0 >> 16);
-                        const uint32_t a2 = e4m3x2_to_f16x2(y0), a3 = e4m3x2_to_f16x2(y0 >> 16);
-                        const uint32_t b0 = e4m3x2_to_f16x2(x1), b1 = e4m3x2_to_f16x2(x1 >> 16);
-                        const uint32_t b2 = e4m3x2_to_f16x2(y1), b3 = e4m3x2_to_f16x2(y1 >> 16);
+            for (int w = 0; w < W; ++w) {
+                if constexpr (C == kE4m3) {
+                    // bytes of two tokens side by side: (token 0, token 1) of values 4w, 4w+1 | 4w+2, 4w+3
+                    const uint32_t x0 = __byte_perm(vw[0][w], vw[1][w], 0x5140), x1 = __byte_perm(vw[0][w], vw[1][w], 0x7362);
+                    const uint32_t y0 = __byte_perm(vw[2][w], vw[3][w], 0x5140), y1 = __byte_perm(vw[2][w], vw[3][w], 0x7362);
+                    const uint32_t a0 = e4m3x2_to_f16x2(x0), a1 = e4m3x2_to_f16x2(x0 >> 16);
+                    const uint32_t a2 = e4m3x2_to_f16x2(y0), a3 = e4m3x2_to_f16x2(y0 >> 16);
+                    const uint32_t b0 = e4m3x2_to_f16x2(x1), b1 = e4m3x2_to_f16x2(x1 >> 16);
+                    const uint32_t b2 = e4m3x2_to_f16x2(y1), b3 = e4m3x2_to_f16x2(y1 >> 16);
 #pragma unroll
-                        for (int nt = 0; nt < NT; ++nt) {
-                            mma_16816<C>(o[nt][2 * w], a0, a1, a2, a3, pf[u][nt][0], pf[u][nt][1]);
-                            mma_16816<C>(o[nt][2 * w + 1], b0, b1, b2, b3, pf[u][nt][0], pf[u][nt][1]);
-                        }
-                    } else {
-                        const uint32_t a0 = __byte_perm(vw[0][w], vw[1][w], 0x5410), a1 = __byte_perm(vw[0][w], vw[1][w], 0x7632);
-                        const uint32_t a2 = __byte_perm(vw[2][w], vw[3][w], 0x5410), a3 = __byte_perm(vw[2][w], vw[3][w], 0x7632);
-#pragma unroll
-                        for (int nt = 0; nt < NT; ++nt) mma_16816<C>(o[nt][w], a0, a1, a2, a3, pf[u][nt][0], pf[u][nt][1]);
+                    for (int nt = 0; nt < NT; ++nt) {
+                        mma_16816<C>(o[nt][2 * w], a0, a1, a2, a3, pf[nt][0], pf[nt][1]);
+                        mma_16816<C>(o[nt][2 * w + 1], b0, b1, b2, b3, pf[nt][0], pf[nt][1]);
                     }
+                } else {
+                    const uint32_t a0 = __byte_perm(vw[0][w], vw[1][w], 0x5410), a1 = __byte_perm(vw[0][w], vw[1][w], 0x7632);
+                    const uint32_t a2 = __byte_perm(vw[2][w], vw[3][w], 0x5410), a3 = __byte_perm(vw[2][w], vw[3][w], 0x7632);
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt) mma_16816<C>(o[nt][w], a0, a1, a2, a3, pf[nt][0], pf[nt][1]);
                 }
             }
         }
