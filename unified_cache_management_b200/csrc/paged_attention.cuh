@@ -11,9 +11,9 @@ namespace ucmr {
 // Workspace: header (device status word first), one arrival counter per CTA, then two partial results per CTA: at most
 // kAttnPartRows rows in all, for either kernel.
 constexpr int kAttnMaxSms = 152;
-constexpr int kAttnMaxCtas = 2 * kAttnMaxSms;
 constexpr size_t kAttnPartRows = (size_t)kAttnMaxSms * 2 * 128;
 constexpr size_t kAttnCounterBytes = 512 * sizeof(int32_t);
+static_assert(kAttnCounterBytes >= 2 * kAttnMaxSms * sizeof(int32_t), "two CTAs per SM");
 
 inline size_t attn_workspace_bytes(int D)
 {
@@ -42,7 +42,7 @@ struct AttnParams {
     int64_t os_t, os_h;
     float* lse;              // [T, Hq] or null
     int32_t* status;         // first word of the workspace
-    int32_t* counters;       // [kAttnMaxCtas], zero between launches
+    int32_t* counters;       // [CTAs], zero between launches
     float* partial;
 };
 
