@@ -1,0 +1,50 @@
+"""GPU: corners of attention over the paged KV cache for many rows: value scales far apart, of 0 and at their floor, rows of
+very small queries, and whole items of 256 rows."""
+import math
+
+import pytest
+import torch
+
+from tests import kv_reference as R
+from tests.test_gpu_kv_operators import BF, FP, _attend, _case, _check, _close, _gen
+
+pytestmark = pytest.mark.gpu
+
+
+def _compare(c, mq, room_of, causal=True):
+    """Against the 64-bit form; room_of: what the fp16 weights may add, per output row, beyond the usual room."""
+    out, lse = _attend(c, mq, causal=causal)
+    torch.cuda.synchronize()
+    want, wlse, room, lroom = R.attention(c["q"], c["k_cache"], c["v_cache"], c["table"], c["seq_lens"], k_scale=c["k_scale"],
+                                          v_scale=c["v_scale"], query_start=c["query_start"], causal=causal)
+    _close(out, want, room + room_of, "out")
+    _close(lse, wlse, lroom, "lse")
+
+
+def _tile_blocks(c, i, tile, bs):
+    """Blocks of request i's token tile (128 tokens)."""
+    return c["table"][i, tile * 128 // bs:(tile + 1) * 128 // bs].long()
+
+
+# A weight is counted from 2^(6 - E) in fp16, 2^E at most twice the largest value scale; half of fp16's smallest step is 2^-25: a
+# token adds at most 448 * 2 * scale * 2^-25 * 2^-6 = 448 * scale * 2^-30, over a sum of weights of 1 or more.
+def _fp16_room(scale, tokens):
+    return 448.0 * scale * tokens * 2.0 ** -30
+
+
+@pytest.mark.parametrize("exponent", [-13, -20, -30])
+@pytest.mark.parametrize("nq", [33, 300])
+def test_tiles_of_scale_zero(cuda_device, exponent, nq):
+    """Whole tiles of 128 tokens whose value scales are all 0 (as the append leaves blocks of zeros), or whose blocks are all
+    missing, at the start, in the middle and at the end of a request: the others' weights keep their bits.  Many tiles per
+    CTA: at least as many items as SMs."""
+    n, bs = 1024, 16
+    b, h = (20, 8) if nq < 128 else (40, 16)
+    c, mq = _case(90 - exponent, [n] * b, [nq] * b, h, h, 64, bs, "e4m3", BF)
+    c["v_scale"][:] = 2.0 ** exponent
+    for i, tiles in enumerate([(0,), (1,), (0, 1), (3,), (4,), (7,), (6, 7), (0, 4, 5), (2, 3, 6), ()] * (b // 10)):
+        for t in tiles:
+            c["v_scale"][_tile_blocks(c, i, t, bs)] = 0.0
+        if i % 20 >= 15 and tiles:
+            c["table"][i, tiles[0] * 8:tiles[0] * 8 + 8] = -1
+    _compare(c, mq, _fp16_room(2.0 ** exponent, n))

@@ -64,7 +64,7 @@ template <int D> struct Sizes {
 struct Meta {
     float tok[2][kTok];              // scales per token, keys and values, for a tile whose scales do not come down to one
     uint32_t valid[4];
-    float scale[2];                  // scale of the whole tile
+    float scale[2];                  // scale of the whole tile; values: 0 if there is nothing but zeros
     int general[2];                  // the scales per token are in use instead
     int bad;                         // tokens before the end are missing
 };
@@ -589,14 +589,18 @@ __global__ void __launch_bounds__(kThreads, 1) tile_kernel(const __grid_constant
                     const float vscale = mt.scale[1];
                     kgen = mt.general[0] != 0;
                     vgen = mt.general[1] != 0;
-                    const int e = max(-100, min(128, (int)((__float_as_uint(vscale) & 0x7fffffffu) >> 23) - 126));
-                    if (e > vexp) {
-                        vdown = vexp == -200 ? 0.f : exp2_fast((float)(vexp - e));
-                        vexp = e;
-                    }
-                    vf = exp2_fast(kShift - (float)vexp);
                     if (!kgen) kf *= mt.scale[0];
-                    if (!vgen) vf *= vscale;
+                    if (__float_as_uint(vscale) == 0) {              // no values but zeros, in the product too: no say in E
+                        vf = 1.f;
+                    } else {
+                        const int e = max(-100, min(128, (int)((__float_as_uint(vscale) & 0x7fffffffu) >> 23) - 126));
+                        if (e > vexp) {
+                            vdown = vexp == -200 ? 0.f : exp2_fast((float)(vexp - e));
+                            vexp = e;
+                        }
+                        vf = exp2_fast(kShift - (float)vexp);
+                        if (!vgen) vf *= vscale;
+                    }
                 }
                 // One scale, and no token missing but at the end: columns from `bound` on are hidden.
                 const bool plain = !kgen && !vgen && kf > 0.f && vf > 0.f && !mt.bad;
@@ -1198,14 +1202,14 @@ __global__ void __launch_bounds__(kThreads, 1) tile_kernel(const __grid_constant
                             }
                             lo = __reduce_min_sync(0xffffffffu, lo);
                             hi = __reduce_max_sync(0xffffffffu, hi);
-                            const bool none = hi == 0;           // no scale but 0: values are zeros, and so are their codes
+                            const bool none = hi == 0;           // no scale but 0, or no block: values become zeros, the scale is 0
                             int fold = none && kind == 1, general = 0;
                             if (!none && (lo != hi || __any_sync(0xffffffffu, zero != 0))) {
                                 fold = !__any_sync(0xffffffffu, odd != 0) && (hi >> 23) - (lo >> 23) <= 15;
                                 general = !fold;
                             }
                             if (lane == 0) {
-                                mt.scale[kind] = none && kind == 1 ? 1.f : __uint_as_float(hi);
+                                mt.scale[kind] = __uint_as_float(hi);
                                 mt.general[kind] = general;
                                 slot.folds[kind] = fold;
                             }
