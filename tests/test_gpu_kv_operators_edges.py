@@ -48,3 +48,19 @@ def test_tiles_of_scale_zero(cuda_device, exponent, nq):
         if i % 20 >= 15 and tiles:
             c["table"][i, tiles[0] * 8:tiles[0] * 8 + 8] = -1
     _compare(c, mq, _fp16_room(2.0 ** exponent, n))
+
+
+@pytest.mark.parametrize("nq", [33, 300])
+@pytest.mark.parametrize("exponents", [(0, -126), (60, -126, 0), (60, -90), (7, -126), (100, -20)])
+def test_value_scales_far_apart(cuda_device, nq, exponents):
+    """Tiles whose value scales differ by more than float32's exponents allow for in a product: a value scale has no say in
+    the weights' sum."""
+    n, bs = 1024, 16
+    b, h = (20, 8) if nq < 128 else (40, 16)
+    c, mq = _case(91, [n] * b, [nq] * b, h, h, 64, bs, "e4m3", FP if nq < 128 else BF)
+    for i in range(b):
+        for t in range(n // 128):
+            c["v_scale"][_tile_blocks(c, i, t, bs)] = 2.0 ** exponents[(t + i) // (1 + i % 3) % len(exponents)]
+    if max(exponents) > 7:
+        c["q"] = c["q"].to(BF)                    # (fp16 results would overflow)
+    _compare(c, mq, _fp16_room(2.0 ** max(exponents), n))

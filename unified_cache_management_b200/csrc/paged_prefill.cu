@@ -602,8 +602,10 @@ __global__ void __launch_bounds__(kThreads, 1) tile_kernel(const __grid_constant
                         if (!vgen) vf *= vscale;
                     }
                 }
-                // One scale, and no token missing but at the end: columns from `bound` on are hidden.
-                const bool plain = !kgen && !vgen && kf > 0.f && vf > 0.f && !mt.bad;
+                // One scale, and no token missing but at the end: columns from `bound` on are hidden.  The factor on the weights
+                // goes into their exponential and is taken out of their sum again: not where it is so small that weights
+                // which the sum needs would vanish (at 2^-60 those below 2^-66 of the reference do).
+                const bool plain = !kgen && !vgen && kf > 0.f && vf >= 0x1p-60f && !mt.bad;
                 const int bound = limit - tok0;
                 float alpha = 1.f;
                 auto raise = [&](float top) {
