@@ -64,3 +64,20 @@ def test_value_scales_far_apart(cuda_device, nq, exponents):
     if max(exponents) > 7:
         c["q"] = c["q"].to(BF)                    # (fp16 results would overflow)
     _compare(c, mq, _fp16_room(2.0 ** max(exponents), n))
+
+
+@pytest.mark.parametrize("nq", [33, 300])
+@pytest.mark.parametrize("dtype", [BF, FP])
+def test_rows_of_tiny_queries(cuda_device, nq, dtype):
+    """Rows whose score factor (a power of two of the row's size times the key scale) underflows, beside rows where it does
+    not: every warp takes one way through a tile."""
+    n, bs = 700, 16
+    b, h = (20, 8) if nq < 128 else (40, 16)
+    c, mq = _case(93, [n - 5 * i for i in range(b)], [nq] * b, h, h, 64, bs, "e4m3", dtype)
+    tiny = 2.0 ** -125 if dtype == BF else 2.0 ** -24          # (the smallest fp16 value)
+    c["q"][::7] = torch.where(c["q"][::7] > 0, tiny, -tiny).to(dtype)
+    for i in range(b):
+        for t in range(5):
+            if (t + i) % 3 == 0:
+                c["k_scale"][_tile_blocks(c, i, t, bs)] = 2.0 ** (-26 if dtype == BF else -126)
+    _compare(c, mq, _fp16_room(float(c["v_scale"].max()), n))

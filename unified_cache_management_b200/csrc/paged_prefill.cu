@@ -604,8 +604,9 @@ __global__ void __launch_bounds__(kThreads, 1) tile_kernel(const __grid_constant
                 }
                 // One scale, and no token missing but at the end: columns from `bound` on are hidden.  The factor on the weights
                 // goes into their exponential and is taken out of their sum again: not where it is so small that weights
-                // which the sum needs would vanish (at 2^-60 those below 2^-66 of the reference do).
-                const bool plain = !kgen && !vgen && kf > 0.f && vf >= 0x1p-60f && !mt.bad;
+                // which the sum needs would vanish (at 2^-60 those below 2^-66 of the reference do).  A warp goes one way as a
+                // whole, since both read the tensor memory together: the factor of a row of tiny queries may be 0 alone.
+                const bool plain = __all_sync(0xffffffffu, !kgen && !vgen && kf > 0.f && vf >= 0x1p-60f && !mt.bad);
                 const int bound = limit - tok0;
                 float alpha = 1.f;
                 auto raise = [&](float top) {
@@ -775,6 +776,7 @@ __global__ void __launch_bounds__(kThreads, 1) tile_kernel(const __grid_constant
             if (writer) {
 #pragma unroll 1
                 for (int c = 0; c < D / 16; ++c) {
+                    __syncwarp();   // (rows that are not there have gone ahead)
                     float o[16];
                     if (holds) {
                         uint32_t r[16];
