@@ -81,3 +81,25 @@ def test_rows_of_tiny_queries(cuda_device, nq, dtype):
             if (t + i) % 3 == 0:
                 c["k_scale"][_tile_blocks(c, i, t, bs)] = 2.0 ** (-26 if dtype == BF else -126)
     _compare(c, mq, _fp16_room(float(c["v_scale"].max()), n))
+
+
+@pytest.mark.parametrize("exponent", [-100, -110, -119, -126])
+@pytest.mark.parametrize("b,h,g,nq", [(3, 2, 4, 1), (5, 2, 4, 4), (3, 2, 4, 30), (20, 8, 1, 33), (40, 16, 1, 300)])
+def test_smallest_value_scales(cuda_device, exponent, b, h, g, nq):
+    """Values down to the append's smallest scale, 2^-126.  Weights are counted from 2^14 (up to 16 rows) or 2^6 over the
+    largest scale, as far as float32 holds that: from 2^126 over 1 at most.  So half of fp16's smallest step is 2^-25 of
+    448 * 2^-126 for a token at least, or what it is for larger scales."""
+    n = 1024
+    c, mq = _case(92 + exponent, [n] * b, [nq] * b, h * g, h, 64, 16, "e4m3", BF)
+    c["v_scale"][:] = 2.0 ** exponent
+    room = max(_fp16_room(2.0 ** exponent, n), 448.0 * 2.0 ** -126 * n * 2.0 ** -25)
+    _compare(c, mq, room)
+    # one token with a weight 2^13 times the others' and nothing but zeros as its value: the result is the others'
+    c["q"][:] = 1.125
+    c["k_cache"].view(torch.uint8).zero_()
+    c["k_scale"][:] = 1.0
+    c["v_cache"].copy_(torch.full_like(c["v_cache"], 448.0, dtype=BF).to(c["v_cache"].dtype))
+    first = c["table"][:, 0].long()
+    c["k_cache"][first, 0] = torch.ones_like(c["k_cache"][first, 0], dtype=BF).to(c["k_cache"].dtype)
+    c["v_cache"].view(torch.uint8)[first, 0] = 0
+    _compare(c, mq, room)

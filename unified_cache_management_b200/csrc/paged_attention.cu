@@ -30,7 +30,8 @@
 // exactly, and so do the queries after a power of two per row.  Scores, softmax and rows are float32; the key scale and the
 // softmax scale are applied to the float32 score.  The probability that multiplies V is rounded to fp16 (half a step: 2^-11)
 // with the value scale folded in, counted from 2^(14 - E), E the exponent of the largest value scale so far: the largest
-// product is 2^14, so probabilities down to 2^-28 of the largest keep all bits and those below 2^-39 are dropped.  A bf16
+// product is 2^14, so probabilities down to 2^-28 of the largest keep all bits and those below 2^-39 are dropped.  (E is -112 at
+// least: 2^(14 - E) and 2^(E - 14) are normal numbers.  Before scales of 2^-126 that leaves a largest product of 1.)  A bf16
 // cache uses bf16 operands (probabilities rounded by 2^-8), an fp16 cache fp16 ones.
 //
 // What bounds it: HBM for 4 rows and long contexts (16 x 131072 tokens, 8 heads of 128, e4m3: 730 us, 5.9 TB/s; 64 x 4096
@@ -556,7 +557,7 @@ __global__ void __launch_bounds__(kDecThreads, DecConfig<D, C, NG>::kCtas)
                 vfac[0] = f[16 + one]; vfac[1] = f[16 + two];
                 big = max(big, max(__float_as_uint(fabsf(vfac[0])), __float_as_uint(fabsf(vfac[1]))));
                 if (!TMA) big = __reduce_max_sync(0xffffffffu, big);   // (the same in all lanes otherwise)
-                const int e = max(-100, min(128, (int)(big >> 23) - 126));  // every scale is below 2^e
+                const int e = max(-112, min(128, (int)(big >> 23) - 126));  // every scale is below 2^e
                 if (e > vexp) {
                     vdown = vexp == -200 ? 0.f : exp2_fast((float)(vexp - e));
                     vexp = e;

@@ -25,7 +25,8 @@
 //
 // The running maximum that the rows refer to is only raised when it is exceeded by 2^8, so O rarely has to be scaled
 // inside TMEM; P is counted from 2^(6 - E) for fp16 (largest product 2^14, all bits kept down to 2^-20 of the row's
-// reference and nothing dropped above 2^-30), E as in paged_attention.cu.
+// reference and nothing dropped above 2^-30), E as in paged_attention.cu but -120 at least (2^(6 - E) and 2^(E - 6) are normal
+// numbers).
 // What bounds it: for many rows the issue of the softmax and of the loaders' conversions beside the tensor core, and the
 // instruction cache between them; Q K^T with both operands in shared memory takes all of its bandwidth while it runs.  2 x
 // 4096 tokens behind 16384, 32 / 8 heads of 128, e4m3: 2.09 ms, 652 TFLOP/s.  For few rows a tile of 128 tokens takes a
@@ -593,7 +594,7 @@ __global__ void __launch_bounds__(kThreads, 1) tile_kernel(const __grid_constant
                     if (__float_as_uint(vscale) == 0) {              // no values but zeros, in the product too: no say in E
                         vf = 1.f;
                     } else {
-                        const int e = max(-100, min(128, (int)((__float_as_uint(vscale) & 0x7fffffffu) >> 23) - 126));
+                        const int e = max(-120, min(128, (int)((__float_as_uint(vscale) & 0x7fffffffu) >> 23) - 126));
                         if (e > vexp) {
                             vdown = vexp == -200 ? 0.f : exp2_fast((float)(vexp - e));
                             vexp = e;
@@ -710,8 +711,8 @@ __global__ void __launch_bounds__(kThreads, 1) tile_kernel(const __grid_constant
                                 const bool seen = tok0 + c * 16 + j + q < limit && ((seen16 >> (j + q)) & 1u);
                                 x[q] = seen ? exp2_fast(x[q] - base) : 0.f;
                                 sum += x[q];
-                                x[q] *= vf;
-                                if (vgen) x[q] = seen ? x[q] * mt.tok[1][c * 16 + j + q] : 0.f;
+                                if (!vgen) x[q] *= vf;
+                                else x[q] = seen ? x[q] * (vf * mt.tok[1][c * 16 + j + q]) : 0.f;   // (vf alone may reach 2^126)
                             }
                             w[j / 2] = pack2<kP>(x[0], x[1]);
                         }
