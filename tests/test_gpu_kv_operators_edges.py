@@ -103,3 +103,104 @@ def test_smallest_value_scales(cuda_device, exponent, b, h, g, nq):
     c["k_cache"][first, 0] = torch.ones_like(c["k_cache"][first, 0], dtype=BF).to(c["k_cache"].dtype)
     c["v_cache"].view(torch.uint8)[first, 0] = 0
     _compare(c, mq, room)
+
+
+def _whole_items(c, hq, hkv, lens, qs):
+    """The rule by which a call takes whole items of 256 rows: at least four per CTA, none above a third of a CTA's share."""
+    ctas = min(152, torch.cuda.get_device_properties(0).multi_processor_count)
+    g = hq // hkv
+    tiles = [-(-nq * g // 256) for nq in qs]
+    units = [max(1, -(-n // 128)) + 4 for n in lens]
+    total = sum(t * u for t, u in zip(tiles, units)) * hkv
+    largest = max(u for u, nq in zip(units, qs) if nq > 0)
+    return sum(tiles) * hkv >= 4 * ctas and 3 * largest * ctas <= total
+
+
+@pytest.mark.parametrize("kind,dtype,d", [("e4m3", BF, 128), ("e4m3", FP, 64), ("e4m3", BF, 64), ("e4m3", FP, 128),
+                                          ("same", BF, 128), ("same", BF, 64), ("same", FP, 128), ("same", FP, 64)])
+@pytest.mark.parametrize("g,per_head,bs", [(1, True, 16), (4, False, 24), (8, True, 128)])
+def test_whole_items(cuda_device, kind, dtype, d, g, per_head, bs):
+    """Items of 256 rows, taken whole: both chains on rows of their own, tails of 128 rows or fewer, rows that see nothing,
+    several query heads per kv head, lists per kv head."""
+    h, b = 8, 56
+    qs = [(260 + 37 * (i % 9)) // g - (i % 5 == 4) * (130 // g) for i in range(b)]
+    lens = [qs[i] + (i * 53) % 400 if i % 7 else qs[i] - 30 // g for i in range(b)]
+    c, mq = _case(d + g, lens, qs, h * g, h, d, bs, kind, dtype, per_head=per_head)
+    assert _whole_items(c, h * g, h, lens, qs)
+    for causal in (True, False):
+        a = _check(c, mq, causal=causal)
+        b2 = _attend(c, mq, causal=causal)
+        assert torch.equal(a[0], b2[0]) and torch.equal(a[1], b2[1])
+
+
+@pytest.mark.parametrize("kind,dtype", [("e4m3", BF), ("e4m3", FP), ("same", BF), ("same", FP)])
+def test_whole_items_masked_places(cuda_device, kind, dtype):
+    """NaN and infinities behind a length and above the diagonal, block ids out of range, in whole items."""
+    from unified_cache_management_b200 import ops
+    h, b, bs, d = 8, 64, 32, 64
+    qs = [290 - (i % 4) * 10 for i in range(b)]
+    lens = [q + (i * 31) % 150 for i, q in enumerate(qs)]
+    c, mq = _case(7, lens, qs, h, h, d, bs, kind, dtype)
+    assert _whole_items(c, h, h, lens, qs)
+    # positions of each cache row: the request and token that it holds
+    token = torch.full(c["k_cache"].shape[:2], 1 << 30, device="cuda")
+    first = torch.full_like(token, 0)
+    for i, n in enumerate(lens):
+        p = torch.arange(n, device="cuda")
+        blk = c["table"][i, p // bs].long()
+        token[blk, p % bs] = p
+        first[blk, p % bs] = n - qs[i]                         # tokens that all of the request's queries see
+    hidden = token == 1 << 30
+    for name in ("k_cache", "v_cache"):
+        x = c[name].float()
+        x[hidden] = math.nan
+        c[name].copy_(x.to(c[name].dtype))
+    odd = (token >= first + 5) & (token % 61 == 7) & ~hidden   # above the diagonal of the first queries at least
+    x = c["v_cache"].float()
+    x[odd, :, 3] = math.nan
+    if kind == "same":
+        x[odd, :, 5] = math.inf
+    c["v_cache"].copy_(x.to(c["v_cache"].dtype))
+    c["table"][3, 1], c["table"][11, 2] = -5, 1 << 20
+    ws = ops.new_attention_workspace(d, "cuda")
+    out, lse = _attend(c, mq, workspace=ws)
+    assert ops.workspace_status(ws) == 1
+    want, wlse, room, lroom = R.attention(c["q"], c["k_cache"], c["v_cache"], c["table"], c["seq_lens"], k_scale=c["k_scale"],
+                                          v_scale=c["v_scale"], query_start=c["query_start"])
+    clean = [j for j in range(d) if j not in (3, 5)]
+    _close(out[..., clean], want[..., clean], room[..., clean], "out")
+    _close(lse, wlse, lroom, "lse")
+    # the odd columns: not finite exactly where the row sees such a token
+    for j in (3, 5) if kind == "same" else (3,):
+        assert torch.equal(out[..., j].isfinite(), want[..., j].isfinite())
+        fine = want[..., j].isfinite()
+        assert fine.any() and not fine.all()
+        _close(out[..., j][fine], want[..., j][fine], room[..., j][fine], "out")
+
+
+@pytest.mark.parametrize("d,dtype", [(64, FP), (128, BF)])
+def test_whole_items_scales(cuda_device, d, dtype):
+    """Scales in whole items: equal within a tile, powers of two that fold into the codes, too far apart for that, no powers
+    of two, zeros."""
+    h, b, bs = 8, 40, 16
+    qs, lens = [280] * b, [400 + (i * 37) % 300 for i in range(b)]
+    c, mq = _case(8, lens, qs, h, h, d, bs, "e4m3", dtype)
+    g = _gen(9)
+    nb = c["v_scale"].shape[0]
+    for name, base in (("k_scale", -7), ("v_scale", -6)):
+        wide = torch.randint(base - 18, base + 1, (nb, h), device="cuda", generator=g).float()
+        near = torch.randint(base - 6, base + 1, (nb, h), device="cuda", generator=g).float()
+        s = torch.pow(2.0, near)
+        for i in range(b):
+            mine = c["table"][i, :-(-lens[i] // bs)].long()
+            if i % 5 == 1:
+                s[mine] = 2.0 ** base
+            elif i % 5 == 2:
+                s[mine] = torch.pow(2.0, wide[mine])
+            elif i % 5 == 3:
+                s[mine] *= 1.0 + torch.rand((len(mine), h), device="cuda", generator=g)
+            elif i % 5 == 4:
+                s[mine[::3]] = 0.0
+        c[name].copy_(s)
+    assert _whole_items(c, h, h, lens, qs)
+    _compare(c, mq, _fp16_room(float(c["v_scale"].max()), max(lens)))
