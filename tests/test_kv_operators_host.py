@@ -110,3 +110,36 @@ def test_rotary_frequencies():
     for bad in (dict(rotary_dim=0), dict(rotary_dim=7), dict(rotary_dim=8, scaling={"type": "odd"}), dict(rotary_dim=8, scaling={"type": "linear", "factor": 0})):
         with pytest.raises(ValueError):
             ops.rotary_frequencies(**bad)
+
+
+def test_yarn_entries():
+    """Every key of a yarn entry counts: the factor from mscale and mscale_all_dim, ends of the ramp that are not rounded."""
+    yarn = {"type": "yarn", "factor": 40, "original_max_position_embeddings": 4096, "beta_fast": 32, "beta_slow": 1}
+    plain, m = ops.rotary_frequencies(64, 10000.0, yarn)
+    assert math.isclose(m, 0.1 * math.log(40.0) + 1.0)
+
+    def s(x):
+        return 0.1 * x * math.log(40.0) + 1.0
+    for one, every in ((0.707, 0.707), (1.0, 1.0), (1.0, 0.5), (0.707, 2.0)):
+        f, m = ops.rotary_frequencies(64, 10000.0, dict(yarn, mscale=one, mscale_all_dim=every))
+        assert math.isclose(m, s(one) / s(every), rel_tol=1e-14) and torch.equal(f, plain)
+    assert ops.rotary_frequencies(64, 10000.0, dict(yarn, mscale=0.707, mscale_all_dim=1.0, attention_factor=1.5))[1] == 1.5
+    assert ops.rotary_frequencies(64, 10000.0, dict(yarn, factor=1.0, mscale=0.707, mscale_all_dim=1.0))[1] == 1.0
+    assert math.isclose(ops.rotary_frequencies(64, 10000.0, dict(yarn, mscale=1.0, mscale_all_dim=0.0))[1], s(1.0))
+    # the ramp runs from the pair of 32 turns to that of 1 turn over the original context: fractional unless truncated
+    f = 10000.0 ** (-2.0 * torch.arange(32, dtype=torch.float64) / 64)
+    lo, hi = (64 * math.log(4096 / (2 * math.pi * t)) / (2 * math.log(10000.0)) for t in (32.0, 1.0))
+    for cut in (True, False):
+        a, b = (math.floor(lo), math.ceil(hi)) if cut else (lo, hi)
+        slow = ((torch.arange(32, dtype=torch.float64) - a) / (b - a)).clamp(0, 1)
+        got, _ = ops.rotary_frequencies(64, 10000.0, dict(yarn, truncate=cut))
+        assert torch.allclose(got, f * (1 - slow) + f / 40 * slow, rtol=1e-14)
+    assert not torch.equal(ops.rotary_frequencies(64, 10000.0, dict(yarn, truncate=False))[0], plain)
+    # keys without a value are not there; what is not handled, contradicts the base or is defined in two ways is refused
+    assert torch.equal(ops.rotary_frequencies(64, 10000.0, dict(yarn, attention_factor=None, mrope_section=None, rope_theta=10000))[0], plain)
+    for bad in (dict(mscale=0.707), dict(mscale_all_dim=1.0), dict(mscale=0.707, mscale_all_dim=0.0), dict(rope_theta=5e5),
+                dict(mrope_section=[16, 24, 24]), dict(alpha=2.0)):
+        with pytest.raises(ValueError):
+            ops.rotary_frequencies(64, 10000.0, dict(yarn, **bad))
+    with pytest.raises(ValueError):
+        ops.rotary_frequencies(64, 10000.0, {"rope_type": "default", "mrope_section": [16, 24, 24]})

@@ -781,17 +781,28 @@ def softmax_topk(repr_blocks: torch.Tensor, q: torch.Tensor, k: int, workspace: 
 # ----------------------------------------------------------------------------------------------
 _TYPES = {torch.bfloat16: _l.BF16, torch.float16: _l.FP16, torch.float8_e4m3fn: _l.E4M3}
 _ROPE_TYPES = ("default", "linear", "dynamic", "llama3", "yarn")
+# what an entry may hold: read for the types that define it; the last three are taken from the caller's arguments or mean nothing
+_ROPE_KEYS = {"rope_type", "type", "factor", "original_max_position_embeddings", "seq_len", "low_freq_factor", "high_freq_factor",
+              "beta_fast", "beta_slow", "truncate", "attention_factor", "mscale", "mscale_all_dim",
+              "rope_theta", "partial_rotary_factor", "finetuned"}
 
 
 def rotary_frequencies(rotary_dim: int, base: float = 10000.0, scaling: Optional[dict] = None, device=None):
     """(inv_freq float64 [rotary_dim/2], mscale) of a model's ``rope_theta`` and ``rope_scaling`` entry: ``rope_type``
     (or ``type``) 'default', 'linear' (factor), 'dynamic' (factor, original_max_position_embeddings, seq_len: the base
     grows with a length beyond the original one), 'llama3' (factor, low_freq_factor, high_freq_factor,
-    original_max_position_embeddings) or 'yarn' (factor, original_max_position_embeddings, beta_fast, beta_slow,
-    attention_factor)."""
+    original_max_position_embeddings) or 'yarn' (factor, original_max_position_embeddings, beta_fast, beta_slow, truncate: whether
+    the ramp's ends are rounded to whole pairs, attention_factor or mscale and mscale_all_dim).  The factor of a 'yarn' entry is
+    attention_factor, or s(mscale) / s(mscale_all_dim) with s(m) = 0.1 m ln(factor) + 1, or s(1) if neither is given (what a
+    model puts on its softmax besides, such as s(mscale_all_dim)^2, goes into the attention's ``scale``).  A key that
+    is not among these is refused, as is a ``rope_theta`` other than ``base``; a key whose value is None is left out."""
     if rotary_dim <= 0 or rotary_dim % 2:
         raise ValueError("rotary_dim must be even and positive")
-    cfg = dict(scaling or {})
+    cfg = {k: v for k, v in (scaling or {}).items() if v is not None}
+    if set(cfg) - _ROPE_KEYS:
+        raise ValueError(f"rope scaling entry with keys that are not handled: {sorted(set(cfg) - _ROPE_KEYS)}")
+    if float(cfg.get("rope_theta", base)) != float(base):
+        raise ValueError(f"the entry's rope_theta {cfg['rope_theta']} is not the base {base}")
     kind = cfg.get("rope_type", cfg.get("type", "default"))
     if kind not in _ROPE_TYPES:
         raise ValueError(f"rope type should be one of {_ROPE_TYPES}, got {kind!r}")
@@ -822,13 +833,30 @@ def rotary_frequencies(rotary_dim: int, base: float = 10000.0, scaling: Optional
 
         def pair_with(turns):  # (fractional) pair that turns this often over the original context
             return rotary_dim * math.log(original / (2.0 * math.pi * turns)) / (2.0 * math.log(base))
-        first = max(math.floor(pair_with(float(cfg.get("beta_fast", 32.0)))), 0)
-        last = min(math.ceil(pair_with(float(cfg.get("beta_slow", 1.0)))), rotary_dim - 1)
+        first, last = pair_with(float(cfg.get("beta_fast", 32.0))), pair_with(float(cfg.get("beta_slow", 1.0)))
+        if cfg.get("truncate", True):
+            first, last = math.floor(first), math.ceil(last)
+        first, last = max(first, 0), min(last, rotary_dim - 1)
         slow = ((i - first) / max(last - first, 0.001)).clamp(0.0, 1.0)
         f = f * (1.0 - slow) + f / factor * slow
-        mscale = cfg.get("attention_factor")
-        mscale = float(mscale) if mscale is not None else (0.1 * math.log(factor) + 1.0 if factor > 1 else 1.0)
+        mscale = _yarn_factor(cfg, factor)
     return f.to(device), mscale
+
+
+def _yarn_factor(cfg: dict, factor: float) -> float:
+    """Factor of a yarn entry on the rotated values.  Where only one of mscale and mscale_all_dim is there, or one is 0,
+    definitions differ: some leave it aside, others take 1 and 0 for what is missing.  Such an entry is refused unless they agree."""
+    if "attention_factor" in cfg:
+        return float(cfg["attention_factor"])
+
+    def s(m):
+        return 0.1 * m * math.log(factor) + 1.0 if factor > 1 else 1.0
+    one, every = float(cfg.get("mscale", 1.0)), float(cfg.get("mscale_all_dim", 0.0))
+    if one and every and "mscale" in cfg:
+        return s(one) / s(every)
+    if s(one) / s(every) != s(1.0):
+        raise ValueError("a yarn entry needs both of mscale and mscale_all_dim, neither 0, or an attention_factor")
+    return s(1.0)
 
 
 def _type_of(name: str, t: torch.Tensor, allowed) -> int:
