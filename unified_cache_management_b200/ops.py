@@ -921,11 +921,34 @@ def _check_rotary(x, positions, inv_freq, out) -> None:
     _same_device(x.device, out=out, positions=positions, inv_freq=inv_freq)
 
 
+class _Rotary(torch.autograd.Function):
+    """The map is linear: its gradient is the transposed map of the gradient, which has a gradient in turn."""
+
+    @staticmethod
+    def forward(ctx, x, positions, inv_freq, interleaved, mscale, transpose):
+        ctx.save_for_backward(positions, inv_freq)
+        ctx.how = dict(interleaved=interleaved, mscale=mscale, transpose=not transpose)
+        return rotary(x, positions, inv_freq, interleaved=interleaved, mscale=mscale, transpose=transpose)
+
+    @staticmethod
+    def backward(ctx, dy):
+        positions, inv_freq = ctx.saved_tensors
+        if dy.stride(2) != 1:              # (an expanded gradient, as of a sum)
+            dy = dy.clone(memory_format=torch.contiguous_format)
+        return rotary(dy, positions, inv_freq, **ctx.how), None, None, None, None, None
+
+
 def rotary(x: torch.Tensor, positions: torch.Tensor, inv_freq: torch.Tensor, *, interleaved: bool = False,
            mscale: float = 1.0, transpose: bool = False, out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """Rotates the first 2 * len(inv_freq) elements of every head of x [T, H, D] (bf16 / fp16) by positions[t] *
     inv_freq; see ``ucmr_rotary``.  ``out`` may be x itself.  ``transpose`` applies the transposed map, which takes the
-    gradient of the output to the gradient of x."""
+    gradient of the output to the gradient of x.  Where x requires grad, so does the result, and its backward pass is that map;
+    such a call has no ``out``, and inv_freq has no gradient."""
+    learned = getattr(inv_freq, "requires_grad", False)
+    if isinstance(x, torch.Tensor) and (x.requires_grad or learned) and torch.is_grad_enabled():
+        if out is not None or learned:
+            raise ValueError("with gradients, out cannot be given, and inv_freq cannot require one")
+        return _Rotary.apply(x, positions, inv_freq, interleaved, mscale, transpose)
     if out is not None or not (isinstance(x, torch.Tensor) and x.is_cuda and x.dtype in _ACTIVATIONS and x.dim() == 3):
         _check_rotary(x, positions, inv_freq, out)
     t, h, d = x.shape
