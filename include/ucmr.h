@@ -422,8 +422,10 @@ int ucmr_softmax_topk(const void* repr, int n_blocks, int M, int Hkv, int D, con
  *         mscale * (a cos - b sin, b cos + a sin) of the angle positions[t] * inv_freq[i],
  *     with the angle negated when transpose != 0 (the transposed map: the gradient, and for mscale = 1 the inverse);
  *     the other elements are copied.  positions int32 or int64 [T], any value; inv_freq float64 [rotary_dim/2] (device,
- *     radians per position; scalings for long contexts go in here and in mscale).  Angles are reduced exactly (64-bit
- *     fractions of a turn): the error of an angle is at most |positions * inv_freq| * 2^-53 + 2^-23.
+ *     radians per position, >= 0; scalings for long contexts go in here and in mscale).  Angles are counted in 64-bit
+ *     fractions of a turn and reduced by wrapping: the error of an angle is at most |positions * inv_freq| * 2^-52 (inv_freq
+ *     over 2 pi in float64) + |positions| * 2 pi * 2^-64 (the fraction cut to 64 bits: 2^-21.3 at position 2^40, the larger
+ *     part for slow pairs) + 2^-23.
  *     float32 arithmetic, one rounding.
  * ------------------------------------------------------------------------------------------ */
 int ucmr_rotary(const void* x, void* out, int64_t T, int H, int D, int64_t x_stride_t, int64_t x_stride_h,

@@ -3,9 +3,11 @@
 // Pair i of a head is turned by the angle position * inv_freq[i].  The angle of a far position does not fit float32
 // (4 Mi * 1 rad has a step of 0.25 rad), so it is counted in turns, as a 64-bit binary fraction: F = inv_freq / 2 pi
 // scaled by 2^64, and position * F modulo 2^64 is the fraction of a turn - the wrap-around of the integer product IS the
-// reduction.  Its top 32 bits, read as a signed number, are the angle in units of pi * 2^-31, for sincospif.  F carries
-// the 53 bits of the double it comes from: the angle is off by at most |position * inv_freq| * 2^-53, plus pi * 2^-25 for
-// the float32 argument (a rounding of half a step at the largest argument, 1), below what a 16-bit result can show.
+// reduction.  Its top 32 bits, read as a signed number, are the angle in units of pi * 2^-31, for sincospif.  Three errors
+// add up.  1 / 2 pi and its product with inv_freq are rounded to float64: off by 2^-53.3 and 2^-53 of themselves, together less
+// than |position * inv_freq| * 2^-52 (inv_freq >= 0; the subtraction of whole turns is exact).  F is cut to 64 bits: at most
+// |position| * 2 pi * 2^-64, which is 2^-21.3 at position 2^40.  The float32 argument: pi * 2^-25, a rounding of half a step at the
+// largest argument, 1, and 2 pi * 2^-32 for the bits below the top 32, together less than 2^-23 (a 16-bit result shows no more).
 // No table of cosines has to be kept or read.
 #pragma once
 
