@@ -445,6 +445,7 @@ int ucmr_rotary(const void* x, void* out, int64_t T, int H, int D, int64_t x_str
  *       NaN and have no say in the scale.
  *     q (may be NULL): the step's queries [T, Hq, D], rotated into q_out (may be q).  k_out (may be NULL, not k): the rotated
  *     keys of all T tokens in 16 bits [T, Hkv, D], for example for ucmr_hash_encode_decode_step.  Both need inv_freq.
+ *     T up to 4194304 (every block's owner looks through the slot list: that part of the time grows with T^2).
  *     D a multiple of 16 up to 512, BS up to 1024, rotary_dim a multiple of 16; k, v and the caches 16-byte aligned with
  *     strides of whole 16-byte vectors.
  * ------------------------------------------------------------------------------------------ */

@@ -143,3 +143,11 @@ def test_yarn_entries():
             ops.rotary_frequencies(64, 10000.0, dict(yarn, **bad))
     with pytest.raises(ValueError):
         ops.rotary_frequencies(64, 10000.0, {"rope_type": "default", "mrope_section": [16, 24, 24]})
+
+
+def test_append_token_limit():
+    """The walk of the slot list grows with the square of the tokens: a call has a limit."""
+    lib = L.load_library()
+    for cache in (dict(), dict(cache=L.BF16, ks=NULL, vs=NULL)):
+        assert _append(lib, T=(1 << 22) + 1, **cache) == L.UCMR_ERR_UNSUPPORTED
+        assert _append(lib, T=1 << 40, **cache) == L.UCMR_ERR_UNSUPPORTED

@@ -20,7 +20,8 @@
 // a slot is listed twice, the later token's row is the one that is stored.  So the result does not depend on the order
 // in which CTAs run, whatever the order of the slot list, and no atomic touches global memory.
 // The walk costs T / chunk * head groups * T slot reads out of L2: 67 MB for 32768 tokens in blocks and chunks of 128 with
-// one head group, next to 740 MB of HBM traffic that such a call (8 + 32 heads of 128, e4m3) cannot do without.
+// one head group, next to 740 MB of HBM traffic that such a call (8 + 32 heads of 128, e4m3) cannot do without.  It grows with the
+// square of T, so a call takes kAppMaxTokens tokens at most (a terabyte of L2 reads).
 //
 // Keys and values of a candidate go to the two halves of the CTA (256 threads each), in turn, since keys take longer.  A half
 // goes over the rows of one head of the block twice, first for the largest value, then, out of L2, for the codes.  Cosines
@@ -42,6 +43,7 @@ constexpr int kAppHalf = 256;              // threads per half
 constexpr int kAppTile = 16384;            // elements of a head whose cosines and sines are in shared memory: 64 KB
 constexpr int kAppMaxChunk = 128;
 constexpr int kAppMaxBlock = 1024;         // rows per block
+constexpr int kAppMaxTokens = 1 << 22;     // per call
 constexpr int kAppList = 1024;             // (candidate, token) pairs that the walk may find before it is repeated per candidate
 
 struct AppendJob {
@@ -506,7 +508,7 @@ extern "C" int ucmr_kv_append(const void* k, int64_t k_stride_t, int64_t k_strid
     if (inv_freq && (rotary_dim <= 0 || rotary_dim % 2 != 0 || rotary_dim > D)) return UCMR_ERR_BAD_ARG;
     if (!inv_freq && (q || k_out)) return UCMR_ERR_BAD_ARG;
     if (D % 16 != 0 || D > 512 || BS > kAppMaxBlock || (inv_freq && rotary_dim % 16 != 0)) return UCMR_ERR_UNSUPPORTED;
-    if (T > 0x7FFFFFFF || NB * (int64_t)BS > ((int64_t)1 << 46)) return UCMR_ERR_UNSUPPORTED;
+    if (T > kAppMaxTokens || NB * (int64_t)BS > ((int64_t)1 << 46)) return UCMR_ERR_UNSUPPORTED;
     if (T == 0) return UCMR_OK;
     if (!k || !v || !slot_mapping || !k_cache || !v_cache || (inv_freq && !positions) || (q && !q_out) || k_out == k) return UCMR_ERR_BAD_ARG;
     // whole 16-byte vectors of every row, in and out
