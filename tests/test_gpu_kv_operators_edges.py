@@ -1,5 +1,5 @@
 """GPU: corners of attention over the paged KV cache for many rows: value scales far apart, of 0 and at their floor, rows of
-very small queries, and whole items of 256 rows."""
+very small queries, whole items of 256 rows, and long runs of rows that see nothing."""
 import math
 
 import pytest
@@ -204,3 +204,21 @@ def test_whole_items_scales(cuda_device, d, dtype):
         c[name].copy_(s)
     assert _whole_items(c, h, h, lens, qs)
     _compare(c, mq, _fp16_room(float(c["v_scale"].max()), max(lens)))
+
+
+@pytest.mark.parametrize("kind,dtype,d", [("e4m3", BF, 128), ("same", FP, 64)])
+@pytest.mark.parametrize("hq,hkv,lens,qs", [
+    (36, 9, [828, 900, 330, 15, 627, 900, 15], [200] * 7),
+    (72, 9, [5, 310, 0, 357, 5, 423, 3], [300] * 6 + [148]),
+    (21, 3, [194, 3, 5, 137, 1, 1, 3, 230, 0, 2, 4, 276, 2, 5, 163, 5], [187, 200, 66, 200, 84, 149, 200, 200, 51, 200, 11, 166, 200, 200, 38, 200]),
+    (8, 2, [700, 3] + [0] * 250 + [129, 0, 0, 0, 0, 0, 0, 1], [33] * 260),          # a batch padded with empty requests
+    (64, 8, [40 + i % 3 for i in range(40)], [200] * 40)])                          # whole items of 256 rows
+def test_many_items_that_see_nothing(cuda_device, kind, dtype, d, hq, hkv, lens, qs):
+    """Long runs of row tiles without a single visible token, behind tiles with some: no role waits for another for ever."""
+    from unified_cache_management_b200 import ops
+    c, mq = _case(len(lens), lens, qs, hq, hkv, d, 16, kind, dtype)
+    ws = ops.new_attention_workspace(d, "cuda")
+    out, lse = _check(c, mq, workspace=ws)
+    assert ops.workspace_status(ws) == 0
+    rows = torch.cat([torch.arange(n, device="cuda") < n - l for l, n in zip(lens, qs)])     # those that see nothing
+    assert (out[rows] == 0).all() and (lse[rows] == -math.inf).all()

@@ -96,6 +96,7 @@ struct TileSlot {
     int end;                         // no tile: the last slot
 };
 constexpr int kNoEdge = 0x7fffffff;
+constexpr uint32_t kNothing = 0xffffffffu;   // scale of a token without a block (a NaN that no arithmetic makes)
 
 // A stretch of an item's token tiles.
 struct Segment {
@@ -117,7 +118,6 @@ struct Shared {
     Meta meta[kMetaSlots];
     TileSlot tile[kTileSlots];
     int entry[2][kTok];              // block-table entries of the tile to be placed and of the one after
-    float scale[2][2][kTok];         // scales of the tile to be settled and of the one after
     float merge_m[128], merge_l[128];
     alignas(8) uint64_t k_full[kStages], k_empty[kStages], v_full[kStages], v_empty[kStages];
     uint64_t s_full[2], p_full[2], o_full[2], q_full;
@@ -1150,44 +1150,39 @@ __global__ void __launch_bounds__(kThreads, 1) tile_kernel(const __grid_constant
                 }
             }
         } else if (warp == 19) {
-            // ============================= scales: asked for when a tile has been placed, used when the next one has ============
-            // (Loops over the lane's four tokens unrolled, unlike the others: verification 153 -> 138 us.)
+            // ============================= scales: once the tile has been placed ===================================
+            // A tile does not wait for the next one to be placed: segments without tiles (rows that see nothing) may follow, more than
+            // the ring holds, and then the planner waits for the softmax, which waits for this tile.  Scales come straight into
+            // registers (verification 112 us; by copies through shared memory, a tile ahead, 131), in loops over the lane's four
+            // tokens that are unrolled, unlike the others.
             // One scale for the tile, keys and values each.  All alike: that one.  Powers of two within 2^15 of one another: the
             // largest, and the codes are multiplied by the quotient on the way to fp16 - exactly, since a code is a multiple
             // of 2^-9 and fp16 holds multiples of 2^-24.  Otherwise the softmax takes the scales token by token.
-            uint32_t tile = 0;
 #pragma unroll 1
-            for (bool more = true, has = false; more || has; ++tile) {
-                if (more) {
-                    wait_ring(sm, &sm.t_placed[tile % kTileSlots], (tile / kTileSlots) & 1, p.status);
-                    const TileSlot& slot = sm.tile[tile % kTileSlots];
-                    more = !slot.end;
-                    if (C == kE4m3 && more) {
+            for (uint32_t tile = 0, end = 0; !end; ++tile) {
+                wait_ring(sm, &sm.t_placed[tile % kTileSlots], (tile / kTileSlots) & 1, p.status);
+                TileSlot& slot = sm.tile[tile % kTileSlots];
+                Meta& mt = sm.meta[tile % kMetaSlots];
+                end = slot.end;
+                if (!end) {
+                    if constexpr (C == kE4m3) {
+                        float of[2][kTok / 32];      // the lane's four tokens'
 #pragma unroll
-                        for (int at = lane; at < kTok; at += 32) {
-                            const int blk = slot.block[at];
+                        for (int i = 0; i < kTok / 32; ++i) {
+                            const int blk = slot.block[lane + 32 * i];
+                            of[0][i] = of[1][i] = __uint_as_float(kNothing);
                             if (blk < 0) continue;
                             const int64_t from = (int64_t)blk * p.Hkv + slot.head;
-                            copy4(&sm.scale[tile & 1][0][at], p.scale[0] + from);
-                            copy4(&sm.scale[tile & 1][1][at], p.scale[1] + from);
+                            of[0][i] = __ldg(p.scale[0] + from);
+                            of[1][i] = __ldg(p.scale[1] + from);
                         }
-                    }
-                }
-                asm volatile("cp.async.commit_group;" ::: "memory");
-                if (has) {                           // the tile before
-                    asm volatile("cp.async.wait_group 1;" ::: "memory");
-                    const uint32_t t = tile - 1;
-                    TileSlot& slot = sm.tile[t % kTileSlots];
-                    Meta& mt = sm.meta[t % kMetaSlots];
-                    if constexpr (C == kE4m3) {
 #pragma unroll 1
                         for (int kind = 0; kind < 2; ++kind) {
-                            const float* of = sm.scale[t & 1][kind];
                             uint32_t lo = 0xffffffffu, hi = 0, odd = 0, zero = 0;
 #pragma unroll
-                            for (int at = lane; at < kTok; at += 32) {
-                                if (slot.block[at] < 0) continue;
-                                const uint32_t b = __float_as_uint(of[at]);
+                            for (int i = 0; i < kTok / 32; ++i) {
+                                const uint32_t b = __float_as_uint(kind ? of[1][i] : of[0][i]);
+                                if (b == kNothing) continue;
                                 if (b == 0) { zero = 1; continue; }
                                 lo = min(lo, b);
                                 hi = max(hi, b);
@@ -1208,8 +1203,10 @@ __global__ void __launch_bounds__(kThreads, 1) tile_kernel(const __grid_constant
                             }
                             if (fold || general) {
 #pragma unroll
-                                for (int at = lane; at < kTok; at += 32) {
-                                    const float v = slot.block[at] < 0 ? 0.f : of[at];
+                                for (int i = 0; i < kTok / 32; ++i) {
+                                    const int at = lane + 32 * i;
+                                    float v = kind ? of[1][i] : of[0][i];
+                                    if (__float_as_uint(v) == kNothing) v = 0.f;
                                     // 2^-d with d up to 15 (the last one subnormal), 0 for 0, twice in fp16
                                     const uint32_t d = (hi >> 23) - (__float_as_uint(v) >> 23);
                                     slot.fold[kind][at] = v == 0.f ? 0u : (d < 15 ? (15 - d) << 10 : 0x200u) * 0x10001u;
@@ -1225,14 +1222,9 @@ __global__ void __launch_bounds__(kThreads, 1) tile_kernel(const __grid_constant
                         if (lane == 0) mt.valid[k] = votes;
                     }
                     if (lane == 0) mt.bad = bad;
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(&sm.t_full[t % kTileSlots]);
                 }
-                has = more;
-                if (!more) {                         // the end goes on to the loaders
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(&sm.t_full[tile % kTileSlots]);
-                }
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&sm.t_full[tile % kTileSlots]);   // (the end goes on to the loaders)
             }
         } else if (warp == 17 && lane == 0) {
             // ============================= scheduler ==============================================================
