@@ -471,6 +471,7 @@ int ucmr_kv_append(const void* k, int64_t k_stride_t, int64_t k_stride_h, const 
  *     disjoint blocks (a sequence-sharded cache) are merged with it.
  *     Tokens of blocks outside [0, NB) are left out and flagged (UCMR_DEV_BAD_BLOCK_ID) in the workspace's status word.
  *     Values in masked places (behind a length, above the diagonal) never reach a result, NaN included.
+ *     Scales are finite and >= 0; a value scale has no say in the weights' sum, however far the scales lie apart.
  *     D is 64 or 128.  q, out, caches: 16-byte aligned, strides of whole 16-byte vectors.
  *     workspace: ucmr_paged_attention_workspace_bytes(D) bytes, cleared once with ucmr_paged_attention_workspace_init (or
  *     zero-filled); calls that may overlap on the GPU need different workspaces.  Results do not depend on timing.

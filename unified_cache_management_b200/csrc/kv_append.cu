@@ -28,9 +28,9 @@
 // and sines of a tile of rows are computed once per block, in shared memory, for all heads.  HBM-bound in principle (2 bytes
 // read and 1 written per element); what it does reach is set by latency and instruction issue: two CTAs of 512 threads fit an
 // SM with 64 registers a thread.  Measured for the call above: 180 us, 84 us of it the queries' rotation (at its floor);
-// 91 us for keys and values without rotation, 136 us with it, where their bytes would take 31 us.  Tried and slower: values
-// held in registers between the passes (234 us in all), halves of 128 threads, one or three CTAs per SM.
-// A decode step of 16 tokens takes 6.5 us on the GPU, bound by latency: walk, filter, rows, two passes.
+// keys and values alone 92 us, 67 us without rotation, where their bytes would take 31 us; four times the tokens 448 us, sixteen
+// times 3570 us, by the walk.  The rotated keys written out besides: 208 us.  Tried and slower: values held in registers between the passes (234 us in all), halves of 128 threads, one or three CTAs per SM.
+// A decode step of 16 tokens takes 7.4 us in a graph (6.0 us for 16-bit caches), bound by latency: walk, filter, rows, two passes.
 #include <cuda_fp8.h>
 
 #include "rotary.cuh"

@@ -1,7 +1,7 @@
 // Attention over the paged KV cache (sm_100a): out = softmax(scale * q k^T) v over the tokens of the blocks that a table
 // lists, for up to 16 rows per (request, kv head): decode steps and short verifications.  Calls with more rows go to
-// paged_prefill.cu (verification of 4 tokens with 8 query heads per kv head, 32 rows: 138 us there, 318 us here in two row
-// tiles; 16 rows, 16 requests of 8192 tokens: 131 us here, 168 us there).  Cache of 16-bit values, or of e4m3 codes with a scale
+// paged_prefill.cu (verification of 4 tokens with 8 query heads per kv head, 32 rows: 112 us there, 205 us here in two row
+// tiles; 16 rows, 16 requests of 8192 tokens: 128 us here, 139 us there).  Cache of 16-bit values, or of e4m3 codes with a scale
 // per (block, kv head).
 //
 // Work.  The G query heads of a kv head times the request's query tokens are rows; 4, 8 or 16 of them (a row tile) share one
@@ -14,7 +14,7 @@
 // Eight warps, each with one of the item's heads and every n-th group of 16 tokens; they do not wait for one another until
 // the item ends.  Each has a ring of stages of 16 tokens in shared memory.  Where a block holds a multiple of 16 tokens, one
 // thread has the copy engine fetch a stage's keys and values (boxes of 16 tokens of a head; a mbarrier tells when they are
-// there): 16 x 131072 tokens 952 -> 710 us against copies by all lanes, which were bound by their instructions.  Otherwise all
+// there): 16 x 131072 tokens 952 -> 735 us in short runs against copies by all lanes, which were bound by their instructions.  Otherwise all
 // lanes copy, 16 bytes at a time, with block ids and tails per token: any block size, any strides.
 //   S^T = K Q^T: tokens are the 16 rows of the matrix instruction, query rows its 8 columns.  The order in which the products
 //     run over the head dimension is free, so each lane takes 16 consecutive bytes of a key (4 lanes per key), and the
@@ -34,10 +34,11 @@
 // least: 2^(14 - E) and 2^(E - 14) are normal numbers.  Before scales of 2^-126 that leaves a largest product of 1.)  A bf16
 // cache uses bf16 operands (probabilities rounded by 2^-8), an fp16 cache fp16 ones.
 //
-// What bounds it: HBM for 4 rows and long contexts (16 x 131072 tokens, 8 heads of 128, e4m3: 730 us, 5.9 TB/s; 64 x 4096
-// tokens in bf16: 180 us, 6.0 TB/s); for 8 and 16 rows of e4m3 the issue of instructions (940 and 1400 us for the former).  Calls
-// of some 10 us of traffic pay 20 to 30 us for the launch, the line, the first copies and the join (16 x 8192 tokens: 70 us
-// for 268 MB).
+// What bounds it: HBM for 16-bit caches (64 x 4096 tokens in bf16, 4 rows: 179 us, 6.0 TB/s); the issue of instructions and
+// their latencies for e4m3, so that time goes with the SM clock: 16 x 131072 tokens, 8 heads of 128, 4 rows, take 735 us (5.8
+// TB/s) in short runs at 1965 MHz and 850 us (5.05 TB/s) in long ones, where the power limit holds the clock near 1.7 GHz (memory
+// clock unchanged); 8 rows 970 us, 16 rows 1350 us.  Calls of some 10 us of traffic pay 20 to 30 us for the launch, the line,
+// the first copies and the join (16 x 8192 tokens: 70 us for 268 MB).
 #include <cuda.h>
 
 #include "paged_attention.cuh"

@@ -10,7 +10,7 @@
 //                    (128-byte swizzle), e4m3 codes converted to fp16 on the way
 //   warp 16          TMEM; one thread issues the products
 //   warp 17          one thread works out the CTA's segments
-//   warps 18, 19     plan the token tiles ahead of the loaders: block table, row offsets, rows on their way into L2; scales
+//   warps 18, 19     plan the token tiles ahead of the loaders: block table, row offsets, rows on their way into L2; then scales
 // Registers are dealt out accordingly: 112 for a softmax thread, 88 for a loader's, 80 for the others.  Between them the
 // roles' loops have to stay in the SM's instruction cache (with twice the unrolling every role ran at half its speed):
 // hence short loops where straight runs would do.
@@ -29,9 +29,9 @@
 // numbers).
 // What bounds it: for many rows the issue of the softmax and of the loaders' conversions beside the tensor core, and the
 // instruction cache between them; Q K^T with both operands in shared memory takes all of its bandwidth while it runs.  2 x
-// 4096 tokens behind 16384, 32 / 8 heads of 128, e4m3: 2.09 ms, 652 TFLOP/s.  For few rows a tile of 128 tokens takes a
-// CTA 4000 to 5500 cycles in any case: 16 requests of 8192 tokens with 20 to 128 rows take 168 to 182 us in e4m3, 121 to 144 us
-// in bf16 (4.4 to 3.7 TB/s); verification of 4 tokens (8 ragged requests up to 65000) 131 us.
+// 4096 tokens behind 16384, 32 / 8 heads of 128, e4m3: 2.13 ms, 643 TFLOP/s.  For few rows a tile of 128 tokens takes a
+// CTA 4000 to 5500 cycles in any case: 16 requests of 8192 tokens with 20 to 128 rows take 140 to 156 us in e4m3, 119 to 150 us
+// in bf16 (4.5 to 3.6 TB/s); verification of 4 tokens (8 ragged requests up to 65000) 112 us.
 // Every wait is bounded: one that gives up sets UCMR_DEV_WAIT_TIMEOUT and an abort flag, after which no role waits any more
 // and all leave by the usual way.
 #include "paged_attention.cuh"

@@ -996,7 +996,7 @@ def kv_append(k: torch.Tensor, v: torch.Tensor, slot_mapping: torch.Tensor, k_ca
     With ``inv_freq`` (and ``positions``) the keys are rotated on the way, the queries ``q`` [T, Hq, D] into ``q_out`` (which
     is returned; made if None), and the rotated keys also go to ``k_out`` in 16 bits (for the hash encode).  Caches of
     k's dtype hold the rows; caches of float8_e4m3fn hold codes, with ``k_scale`` / ``v_scale`` float32 [NB, Hkv].  See
-    ``ucmr_kv_append`` for how a block's scale starts and grows."""
+    ``ucmr_kv_append`` for how a block's scale starts and grows.  There is no gradient."""
     if not _plain_append(k, v, slot_mapping, k_cache, v_cache, k_scale, v_scale, positions, inv_freq, q, q_out, k_out):
         _check_append(k, v, slot_mapping, k_cache, v_cache, k_scale, v_scale, positions, inv_freq, q, q_out, k_out)
     t, hkv, d = k.shape
@@ -1120,7 +1120,9 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     [B] - a request's own, or ``Retrieval.physical`` and ``Retrieval.new_seq_lens`` (with the last block among the
     chosen).  One query token per request (T = B), or request b's tokens at query_start[b] .. query_start[b+1] with
     ``max_query_len`` at least the largest count.  ``scale`` defaults to 1 / sqrt(D).  Returns out, or (out, lse) when the
-    log-sum-exp (float32 [T, Hq]) is wanted.  Rows outside every request are left as they were."""
+    log-sum-exp (float32 [T, Hq]) is wanted.  Rows outside every request are left as they were (in an ``out`` made here: not
+    set).  Without ``workspace`` a call makes and clears one, and block ids out of range, which are left out, go unreported:
+    ``workspace_status`` of a workspace of the caller's tells of them.  There is no gradient."""
     if not _plain_attention(q, k_cache, v_cache, block_table, seq_lens, k_scale, v_scale, query_start, max_query_len, out, lse, workspace):
         _check_attention(q, k_cache, v_cache, block_table, seq_lens, k_scale, v_scale, query_start, max_query_len, out, lse, workspace)
     t, hq, d = q.shape
