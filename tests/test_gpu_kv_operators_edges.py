@@ -222,3 +222,45 @@ def test_many_items_that_see_nothing(cuda_device, kind, dtype, d, hq, hkv, lens,
     assert ops.workspace_status(ws) == 0
     rows = torch.cat([torch.arange(n, device="cuda") < n - l for l, n in zip(lens, qs)])     # those that see nothing
     assert (out[rows] == 0).all() and (lse[rows] == -math.inf).all()
+
+
+@pytest.mark.parametrize("kind", ["e4m3", "same"])
+def test_many_requests_and_long_ones(cuda_device, kind):
+    """More requests than threads look at, empty ones among them; one request whose few row tiles are cut over the whole GPU."""
+    from unified_cache_management_b200 import ops
+    ws = ops.new_attention_workspace(64, "cuda")
+    lens = [(i * 37) % 60 if i % 5 else 0 for i in range(1500)]
+    c, mq = _case(94, lens, [1 + i % 2 for i in range(1500)], 20, 1, 64, 16, kind, BF)
+    _check(c, mq, workspace=ws)
+    c, mq = _case(95, [90001], [33], 4, 2, 64, 64, kind, BF)
+    _check(c, mq, workspace=ws)
+    assert ops.workspace_status(ws) == 0
+
+
+def test_many_rows_captured(cuda_device):
+    """Two graphs with a workspace each, replayed side by side, with other lengths and other splits of the query tokens than
+    they were captured with."""
+    from unified_cache_management_b200 import ops
+    c, mq = _case(96, [900, 3000, 50, 400], [40, 1, 30, 29], 8, 2, 128, 16, "e4m3", BF)
+    outs, graphs, streams = [], [], []
+    for _ in range(2):
+        st, ws = torch.cuda.Stream(), ops.new_attention_workspace(128, "cuda")
+        out, lse = torch.empty_like(c["q"]), torch.empty((100, 8), device="cuda")
+        torch.cuda.synchronize()
+        gr = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(gr, stream=st):
+            _attend(c, mq, workspace=ws, out=out, lse=lse)
+        outs.append((out, lse, ws)), graphs.append(gr), streams.append(st)
+    for lens, starts in (((900, 3000, 50, 400), (0, 40, 41, 71, 100)), ((1, 2999, 0, 399), (0, 40, 41, 71, 100)),
+                         ((0, 0, 50, 0), (0, 25, 50, 75, 100)), ((333, 70, 7, 129), (0, 97, 98, 99, 100))):
+        c["seq_lens"].copy_(torch.tensor(lens, dtype=torch.int32))
+        c["query_start"].copy_(torch.tensor(starts, dtype=torch.int32))
+        torch.cuda.synchronize()
+        for _ in range(3):
+            for st, gr in zip(streams, graphs):
+                with torch.cuda.stream(st):
+                    gr.replay()
+        torch.cuda.synchronize()
+        want, wlse = _check(c, 97)
+        for out, lse, ws in outs:
+            assert torch.equal(out, want) and torch.equal(lse, wlse) and ops.workspace_status(ws) == 0
